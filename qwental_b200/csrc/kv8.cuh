@@ -1,0 +1,92 @@
+// Codes and rows of the 8-bit key-value cache, device side.
+#pragma once
+#include "common.cuh"
+#include "kv8.h"
+#include <cuda_fp8.h>
+
+namespace qw {
+
+template <int FMT>
+__device__ __forceinline__ constexpr float kv8_largest() {
+    return FMT == QW_KV8_E4M3 ? 448.f : 127.f;
+}
+// An e4m3 code's bits, moved one place down behind the sign, are the fp16 number 2^-8 times its value: exact, subnormal codes too, and never a NaN
+// (0x7f becomes 480 * 2^-8).  An int8 code becomes its value.  KV8_UNIT * the fp16 number is what the code stands for.
+template <int FMT>
+__device__ __forceinline__ constexpr float kv8_unit() {
+    return FMT == QW_KV8_E4M3 ? 256.f : 1.f;
+}
+// Two codes, in the upper bytes of the two halves of v, as fp16 numbers (e4m3).
+__device__ __forceinline__ uint32_t kv8_e4m3_half2(uint32_t v) { return ((v >> 1) & 0x3f803f80u) | (v & 0x80008000u); }
+// Two codes plus 128, in the lower bytes of the two halves of v whose upper bytes are 0x64 (1024 + byte), as fp16 numbers (int8).
+__device__ __forceinline__ uint32_t kv8_int8_half2(uint32_t v) {
+    const __half2 h = __hsub2(*(const __half2 *)&v, __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));  // 1152
+    return *(const uint32_t *)&h;
+}
+// Four codes -> fp16 pairs (0, 1) and (2, 3)
+template <int FMT>
+__device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t &h01, uint32_t &h23) {
+    if (FMT == QW_KV8_E4M3) {
+        h01 = kv8_e4m3_half2(__byte_perm(w, 0, 0x1404));
+        h23 = kv8_e4m3_half2(__byte_perm(w, 0, 0x3424));
+    } else {
+        w ^= 0x80808080u;
+        h01 = kv8_int8_half2(__byte_perm(w, 0x64646464u, 0x4140));
+        h23 = kv8_int8_half2(__byte_perm(w, 0x64646464u, 0x4342));
+    }
+}
+template <int FMT>
+__device__ __forceinline__ void kv8_decode4(uint32_t w, float (&x)[4]) {
+    uint32_t a, b;
+    kv8_halves<FMT>(w, a, b);
+    const float2 f = __half22float2(*(const __half2 *)&a), g = __half22float2(*(const __half2 *)&b);
+    x[0] = f.x * kv8_unit<FMT>(), x[1] = f.y * kv8_unit<FMT>(), x[2] = g.x * kv8_unit<FMT>(), x[3] = g.y * kv8_unit<FMT>();
+}
+// Two numbers within the format's range -> two codes in the low bytes, to nearest, ties to even.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_encode2(float a, float b) {
+    if (FMT == QW_KV8_E4M3) return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    return ((uint32_t)__float2int_rn(a) & 0xff) | ((uint32_t)__float2int_rn(b) & 0xff) << 8;
+}
+
+__device__ __forceinline__ float kv8_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float kv8_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T kv8_round(float x);
+template <>
+__device__ __forceinline__ __half kv8_round<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 kv8_round<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// E (2, 4 or 8) consecutive 2-byte values: one load or store where the address allows it (strides are the caller's), else one each.
+template <int E>
+struct Kv8Pack;
+template <> struct Kv8Pack<2> { typedef uint32_t t; };
+template <> struct Kv8Pack<4> { typedef uint2 t; };
+template <> struct Kv8Pack<8> { typedef uint4 t; };
+template <int E, class T>
+__device__ __forceinline__ void kv8_load(const T *p, float *x) {
+    typedef typename Kv8Pack<E>::t P;
+    union { P v; T e[E]; };
+    if (((uintptr_t)p & (2 * E - 1)) == 0) v = __ldcg((const P *)p);
+    else {
+#pragma unroll
+        for (int i = 0; i < E; i++) e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++) x[i] = kv8_float(e[i]);
+}
+template <int E, class T>
+__device__ __forceinline__ void kv8_store(T *p, const float *x) {
+    typedef typename Kv8Pack<E>::t P;
+    union { P v; T e[E]; };
+#pragma unroll
+    for (int i = 0; i < E; i++) e[i] = kv8_round<T>(x[i]);
+    if (((uintptr_t)p & (2 * E - 1)) == 0) *(P *)p = v;
+    else {
+#pragma unroll
+        for (int i = 0; i < E; i++) p[i] = e[i];
+    }
+}
+
+}  // namespace qw
