@@ -89,4 +89,32 @@ __device__ __forceinline__ void kv8_store(T *p, const float *x) {
     }
 }
 
+// Eight consecutive 2-byte values as four words, whatever the address.
+template <class T>
+__device__ __forceinline__ void kv8_load_raw8(const T *p, uint32_t (&w)[4]) {
+    const uint16_t *u = (const uint16_t *)p;
+    if (((uintptr_t)p & 15) == 0) {
+        const uint4 v = __ldcg((const uint4 *)p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = (uint32_t)__ldcg(u + 2 * i) | (uint32_t)__ldcg(u + 2 * i + 1) << 16;
+    }
+}
+template <class T>
+__device__ __forceinline__ float2 kv8_float2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 kv8_float2<__half>(uint32_t w) { return __half22float2(*(const __half2 *)&w); }
+template <>
+__device__ __forceinline__ float2 kv8_float2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+__device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 }  // namespace qw
