@@ -17,7 +17,7 @@ struct AttnArgs {
     const void *q, *gate;
     void *y;
     const int32_t *lens, *slots, *blocks;
-    float *part;  // [nb][max_chunks][qh][hd + 4]: sum w code, then M, m, l, unused
+    float *part;  // [nb][max_chunks][qh][hd] sums of w code, then [nb][qh][max_chunks] of M, m, l, unused
     int64_t q_row, q_head, g_row, g_head, y_row, y_head;
     float scale2;  // softmax scale * log2(e)
     uint32_t nb, qh, G, max_len, nblocks, max_chunks;
@@ -29,6 +29,10 @@ __device__ __forceinline__ uint32_t row_tokens(const Kv8Dev &c, const AttnArgs &
     if (a.slots[r] < 0 || len <= 0) return 0;
     const uint32_t n = min((uint32_t)len, a.max_len);
     return a.blocks ? min(a.nblocks, (n + c.block - 1) / c.block) * c.block : n;
+}
+
+__device__ __forceinline__ float4 *stats_of(const AttnArgs &a, uint32_t hd, uint32_t r, uint32_t qh) {
+    return (float4 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
 }
 
 // Four channels of a head's result: times f, times sigmoid(gate), rounded once.
@@ -435,9 +439,8 @@ __global__ void __launch_bounds__(256, 2) kv8_attn_k(const __grid_constant__ CUt
                     const uint32_t qh = k.h * a.G + head, ch0 = 32 * dg + 4 * g;
                     constexpr float unit = kv8_unit<FMT>();
                     if (k.nch > 1) {
-                        float *p = a.part + (((size_t)k.r * a.max_chunks + k.ch) * a.qh + qh) * (HD + 4);
-                        *(float4 *)(p + ch0) = make_float4(v.x * unit, v.y * unit, v.z * unit, v.w * unit);
-                        if (dg == 0 && g == 0) *(float4 *)(p + HD) = make_float4(M[nt][d], m[nt][d], lt, 0.f);
+                        *(float4 *)(a.part + (((size_t)k.r * a.max_chunks + k.ch) * a.qh + qh) * HD + ch0) = make_float4(v.x * unit, v.y * unit, v.z * unit, v.w * unit);
+                        if (dg == 0 && g == 0) stats_of(a, HD, k.r, qh)[k.ch] = make_float4(M[nt][d], m[nt][d], lt, 0.f);
                     } else finish<T>(a, k.r, qh, ch0, v, poison || lt != lt ? __uint_as_float(0x7fffffffu) : M[nt][d] == -INFINITY ? 0.f : exp2f(M[nt][d] - m[nt][d]) * unit / lt);
                 }
         }
@@ -452,52 +455,57 @@ __global__ void __launch_bounds__(256, 2) kv8_attn_k(const __grid_constant__ CUt
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// A block per (head, row): hd / 4 threads take four channels each of every 1024 / hd-th chunk.  grid (qh, nb) x 256
+// A block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  Bound: the latency of
+// two rounds of loads -- a first form with a block per head went through 188 chunks (48000 tokens) in 47 dependent rounds.  grid (qh hd / 64, nb) x 256
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
-    constexpr uint32_t TC = HD / 4, NG = 256 / TC;
-    __shared__ float4 accs[NG][TC];
-    __shared__ float wm[8][3], lsum[NG];
+    __shared__ float4 accs[16][16];
+    __shared__ float wm[8][2], wl[8];
     pdl_sync();
-    const uint32_t qh = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % TC, cg = tid / TC;
+    const uint32_t qh = blockIdx.x / (HD / 64), ch = blockIdx.x % (HD / 64) * 64, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % 16, cg = tid / 16;
     const uint32_t n = row_tokens(c, a, r), nch = (n + CHUNK - 1) / CHUNK;
     if (nch < 2) return;  // written by the core
-    const float *base = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * (HD + 4);
-    const size_t cs = (size_t)a.qh * (HD + 4);
-    float m = -INFINITY, M = -INFINITY, nan = 0.f;
+    const float4 *st = stats_of(a, HD, r, qh);
+    float m = -INFINITY, M = -INFINITY;
     for (uint32_t k = tid; k < nch; k += 256) {
-        const float Mk = __ldcg(base + k * cs + HD), mk = __ldcg(base + k * cs + HD + 1), lk = __ldcg(base + k * cs + HD + 2);
-        m = fmaxf(m, mk);
-        M = fmaxf(M, Mk);
-        if (lk != lk) nan = 1.f;
+        const float4 s = __ldcg(st + k);
+        M = fmaxf(M, s.x);
+        m = fmaxf(m, s.y);
     }
-    m = warp_max(m), M = warp_max(M), nan = warp_max(nan);
-    if (lane == 0) wm[warp][0] = m, wm[warp][1] = M, wm[warp][2] = nan;
+    m = warp_max(m), M = warp_max(M);
+    if (lane == 0) wm[warp][0] = m, wm[warp][1] = M;
     __syncthreads();
-    for (int w = 0; w < 8; w++) m = fmaxf(m, wm[w][0]), M = fmaxf(M, wm[w][1]), nan = fmaxf(nan, wm[w][2]);
+#pragma unroll
+    for (int w = 0; w < 8; w++) m = fmaxf(m, wm[w][0]), M = fmaxf(M, wm[w][1]);
     float l = 0.f;
+    for (uint32_t k = tid; k < nch; k += 256) {
+        const float4 s = __ldcg(st + k);
+        l += s.y == -INFINITY ? s.z : s.z * exp2f(s.y - m);  // (0, or NaN, where a chunk has no maximum)
+    }
+    l = warp_sum(l);
+    if (lane == 0) wl[warp] = l;
+    const float4 *p = (const float4 *)(a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch) + wc;
+    const size_t cs = (size_t)a.qh * (HD / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t k = cg; k < nch; k += NG) {
-        const float *p = base + k * cs;
-        const float Mk = __ldcg(p + HD), mk = __ldcg(p + HD + 1), lk = __ldcg(p + HD + 2);
-        const float4 v = __ldcg((const float4 *)p + wc);
-        const float w = Mk == -INFINITY ? 0.f : exp2f(Mk - M);
-        if (mk != -INFINITY) l = fmaf(lk, exp2f(mk - m), l);
+#pragma unroll 8
+    for (uint32_t k = cg; k < nch; k += 16) {
+        const float Mk = __ldcg(&st[k].x), w = Mk == -INFINITY ? 0.f : exp2f(Mk - M);
+        const float4 v = __ldcg(p + k * cs);
         acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
     }
     accs[cg][wc] = acc;
-    if (wc == 0) lsum[cg] = l;
     __syncthreads();
-    if (tid >= TC) return;
-    l = lsum[0];
+    if (tid >= 16) return;
+    l = wl[0];
 #pragma unroll
-    for (uint32_t g = 1; g < NG; g++) {
+    for (int w = 1; w < 8; w++) l += wl[w];
+#pragma unroll
+    for (int g = 1; g < 16; g++) {
         const float4 v = accs[g][tid];
         acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-        l += lsum[g];
     }
     const bool bad = (uint32_t)a.lens[r] > a.max_len;
-    finish<T>(a, r, qh, 4 * tid, acc, nan > 0.f || bad ? __uint_as_float(0x7fffffffu) : M == -INFINITY ? 0.f : exp2f(M - m) / l);
+    finish<T>(a, r, qh, ch + 4 * tid, acc, l != l || bad ? __uint_as_float(0x7fffffffu) : M == -INFINITY ? 0.f : exp2f(M - m) / l);
 }
 
 // Which kernel: by the format, the type of rows, and whether 8 or 16 heads share a kv head.
@@ -563,7 +571,7 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     const uint64_t most = (uint64_t)a->nb * mc * c->kvh, fit = 2 * (uint64_t)kv8_sm_count();
     e = qw_launch(L.core, (uint32_t)(most < fit ? most : fit), 256, L.smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess || mc < 2) return e;
-    return qw_launch(L.merge, dim3(a->qh, a->nb), 256, 0, st, d, k);
+    return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
 }
 
 cudaError_t launch_kv8_attn(const QwLaunch &L) {
