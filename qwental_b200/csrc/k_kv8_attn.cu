@@ -1,38 +1,46 @@
-// Attention of one new token per row over the 8-bit key-value cache: split over chunks of 256 tokens, joined by kv8_merge_k.
+// Attention of one new token per row over the 8-bit key-value cache: split over chunks of its tokens, joined by kv8_merge_k.
 //
 //   s_t = scale q . k_t          k_t = code * ks_t: the dot product of q and the codes, times ks_t
-//   y   = sum_t 2^(s'_t - m) vs_t code_t / sum_t 2^(s'_t - m),   s' = s log2(e)
-// A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with a running maximum M of its own, so that the weights of the codes are at
-// most 1 whatever the scales are.  A chunk leaves sum w_t code_t, M, m and l = sum 2^(s'_t - m) in fp32; the join is
-//   y = 2^(M* - m*) sum_c 2^(M_c - M*) acc_c / sum_c 2^(m_c - m*) l_c      with M*, m* the maxima over the chunks, in the order of the chunks.
+//   y   = sum_t 2^(s'_t) vs_t code_t / sum_t 2^(s'_t),   s' = s log2(e)
+// A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with a running maximum M of s' + log2 vs, so that the weights of the codes are at
+// most 1 whatever the scales are; p_t = 2^(s'_t - M) is w_t / vs_t, at most 2^110.  A chunk leaves sum w_t code_t, M and l = sum p_t in fp32; the join is
+//   y = sum_c 2^(M_c - M*) acc_c / sum_c 2^(M_c - M*) l_c      with M* the maximum over the chunks, in the order of the chunks.
 #include "kv8.cuh"
 #include "tmap.cuh"
 
 using namespace qw;
 
 namespace {
-constexpr uint32_t CHUNK = 256;
+// Tokens of a chunk, by the tokens of its row alone (a row's result does not depend on the others of a call): short rows in small pieces, for their latency;
+// a chunk of 256 leaves 6 % of its own bytes as fp32 sums.
+__host__ __device__ inline uint32_t chunk_of(uint32_t n) { return n <= 512 ? 32 : n <= 2048 ? 64 : n <= 8192 ? 128 : 256; }
+__host__ __device__ inline uint32_t chunks_in(uint32_t n) { return (n + chunk_of(n) - 1) / chunk_of(n); }
+constexpr float LOWEST = 7.7037197775489434e-34f, LOWEST_LOG2 = -110.f;  // 2^-110
 
 struct AttnArgs {
     const void *q, *gate;
     void *y;
     const int32_t *lens, *slots, *blocks;
-    float *part;  // [nb][max_chunks][qh][hd] sums of w code, then [nb][qh][max_chunks] of M, m, l, unused
+    float *part;  // [nb][max_chunks][qh][hd] sums of w code, then [nb][qh][max_chunks] of M, l
     int64_t q_row, q_head, g_row, g_head, y_row, y_head;
     float scale2;  // softmax scale * log2(e)
     uint32_t nb, qh, G, max_len, nblocks, max_chunks;
 };
 
-// Tokens, or entries' tokens, that a row goes over (0: none or not in use), and whether its length is one the call allows.
-__device__ __forceinline__ uint32_t row_tokens(const Kv8Dev &c, const AttnArgs &a, uint32_t r) {
-    const int len = a.lens[r];
-    if (a.slots[r] < 0 || len <= 0) return 0;
+// Tokens, or entries' tokens, that a row goes over (0: none or not in use).
+__device__ __forceinline__ uint32_t row_tokens(const Kv8Dev &c, const AttnArgs &a, int slot, int len) {
+    if (slot < 0 || len <= 0) return 0;
     const uint32_t n = min((uint32_t)len, a.max_len);
     return a.blocks ? min(a.nblocks, (n + c.block - 1) / c.block) * c.block : n;
 }
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x: 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
-__device__ __forceinline__ float4 *stats_of(const AttnArgs &a, uint32_t hd, uint32_t r, uint32_t qh) {
-    return (float4 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
+__device__ __forceinline__ float2 *stats_of(const AttnArgs &a, uint32_t hd, uint32_t r, uint32_t qh) {
+    return (float2 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
 }
 
 // Four channels of a head's result: times f, times sigmoid(gate), rounded once.
@@ -49,407 +57,441 @@ __device__ __forceinline__ void finish(const AttnArgs &a, uint32_t r, uint32_t q
 }
 
 // ------------------------------------------------------------------------------------------------ core
-// Persistent blocks of 8 warps; the (row, kv head, chunk) tasks of the launch are numbered in this order and a block takes a run of consecutive ones, so
-// that the queries change rarely.  A task goes by tiles of TOK tokens, whose codes come by 2-D tiled copies (swizzled) into a ring of three slots, K and V
-// in turn, with the scales of both beside K:
-//   scores   S[16 tokens][8 heads] = codes[16][HD] . q^T     mma m16n8k16, a warp per 16 tokens.  Which channel is which k of the product is free as long as
-//            both sides agree, so a lane takes 16 codes with one shared-memory load and they feed four products as they lie.
-//   maxima   of the block's warps through shared memory, then the weights w as fp16 high part and remainder (22 bits)
-//   values   O^T[32 channels][8 heads] += codes^T[32][16 tokens] . w^T: a warp has 32 channels and (for HD < 256) its share of the tokens; four bytes of
-//            four tokens give the operands of two 16-channel products after byte permutations.  No sum crosses warps for HD = 256.
-// Codes become fp16 numbers exactly (kv8.cuh), queries are scaled by a power of two of their own first, so the products are exact and the sums fp32.
-// Two barriers per tile; the loads of the next tile leave right behind the first one.
-template <int HD, int NT>
+// Independent warps: the (row, kv head, chunk) tasks of the launch are numbered in this order, each with as many steps of 32 tokens as it has, and a warp
+// takes those that start within its share of all steps.  It owns a task completely -- queries, running maximum and the sums of all channels in registers --
+// and feeds itself through a ring of K and V tiles with an mbarrier each, so warps wait for nothing but their own copies and overlap one another.
+//   scores   S[16 tokens][8 heads] = codes[16][HD] . q^T     mma m16n8k16.  Which channel is which k of the product is free as long as both sides agree, so a
+//            lane takes 16 codes with one shared-memory load and they feed four products as they lie.
+//   values   O^T[16 channels][8 heads] += codes^T[16][16 tokens] . w^T     a lane takes 16 codes of four tokens; byte permutations pair the tokens; the weights
+//            change lanes by shuffles and travel as fp16 high part and remainder (22 bits).
+// Codes become fp16 numbers exactly (kv8.cuh), queries are divided by a power of two of their own first, so the products are exact and the sums fp32.
+// Measured for 16 ragged rows of 1K to 48K tokens (210 MB, e4m3) against forms that were left: blocks of 8 warps that share a tile of 128 tokens, with two
+// barriers per tile, 87 us (scaling, maxima and barriers of a tile 2800 cycles, one after the other); e4m3 operands as they are (mma m16n8k32) no faster, that
+// product being converted to fp16 ones by the assembler at every use (19 cycles instead of 8).
+constexpr uint32_t STEP = 32;
+
+template <int HD, int NT, bool FEW>
 struct Core {
-    static constexpr int TOK = HD == 256 ? 128 : HD == 128 && NT == 2 ? 128 : 256;
     static constexpr int BOX = HD < 128 ? HD : 128, HALVES = HD / BOX;  // bytes of a row in a copy, copies side by side
-    static constexpr int MT = TOK / 128;             // 16-token tiles of a warp
-    static constexpr int DG = HD / 32, TG = 8 / DG;  // groups of 32 channels, shares of the tokens
-    static constexpr int KS = TOK / 16 / TG;         // 16-token steps of a warp's share
-    static constexpr int SLOT = TOK * HD;
-    // shared memory behind the slots
-    static constexpr int SCALES = 3 * SLOT, P = SCALES + 3 * 2 * TOK * 4, WMAX = P + TOK / 16 * NT * 512, LSUM = WMAX + 8 * NT * 8 * 8, INFO = LSUM + 8 * NT * 8 * 4,
-                         BARS = INFO + 64, FIRST = BARS + 32, BYTES = FIRST + (KV8_MAX_ROWS + 1) * 4 + 1024;
+    static constexpr int TILE = STEP * HD;                              // K or V
+    static constexpr int RING = (FEW ? 3 : 1) * 256 / HD;               // tiles of either: 16 KB per warp, or 48
+    static constexpr int BLOCKS = FEW ? 1 : NT == 1 ? 3 : 2;            // per SM: what shared memory and registers allow
+    static constexpr int CH = HALVES * (HD < 128 ? 4 : 8);              // 16-channel tiles
+    static constexpr int LANE = HD < 128 ? 8 : 16;                      // channels of a lane in a row of a copy
+    // shared memory behind the tiles; then 12 bytes per row
+    static constexpr int SCALES = 4 * RING * 2 * TILE, INFO = SCALES + 4 * RING * 2 * STEP * 4, BARS = INFO + 4 * RING * 32, ROWS = BARS + 4 * RING * 16, BYTES = ROWS + 1024 + 16;
 };
 
-template <int HD, int FMT, class T, int NT>
-__global__ void __launch_bounds__(256, 2) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
-    typedef Core<HD, NT> X;
-    constexpr int TOK = X::TOK, MT = X::MT;
+template <int HD, int FMT, class T, int NT, bool FEW>
+__global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
+    typedef Core<HD, NT, FEW> X;
+    constexpr int RING = X::RING;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    const uint32_t base = smem_u32(smem);
+    uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // swizzled copies need it
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    uint32_t *first = (uint32_t *)(smem + X::FIRST), *info = (uint32_t *)(smem + X::INFO);
-    float *wmax = (float *)(smem + X::WMAX), *lsum = (float *)(smem + X::LSUM);
-    uint64_t *full = (uint64_t *)(smem + X::BARS);
-    if (tid == 0) {
-        for (int i = 0; i < 3; i++) mbar_init(&full[i], 1);
+    const uint32_t Kb = smem_u32(smem) + warp * RING * 2 * X::TILE, Vb = Kb + RING * X::TILE;
+    float *scales = (float *)(smem + X::SCALES) + warp * RING * 2 * STEP;
+    uint4 *info = (uint4 *)(smem + X::INFO) + warp * RING * 2;
+    uint64_t *kbar = (uint64_t *)(smem + X::BARS) + warp * RING * 2, *vbar = kbar + RING;
+    uint32_t *first = (uint32_t *)(smem + X::ROWS), *lenv = first + a.nb + 1, *slotv = lenv + a.nb;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 2 * RING; i++) mbar_init(&kbar[i], 1);
         mbar_init_fence();
     }
     pdl_sync();
-    // ---- chunks of every row, running sum: row r owns numbers first[r] .. first[r + 1] - 1
+    // ---- rows: steps of one kv head, running sum; length (top bit: longer than the call allows), slot
     {
-        uint32_t n[4], s = 0;
+        uint32_t n[8], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t r = tid * 4 + i;
-            n[i] = r < a.nb ? (row_tokens(c, a, r) + CHUNK - 1) / CHUNK : 0;
-            s += n[i];
+        for (int i = 0; i < 8; i++) {
+            const uint32_t r = tid * 8 + i;
+            n[i] = 0;
+            if (r < a.nb) {
+                const int len = a.lens[r], slot = a.slots[r];
+                n[i] = (row_tokens(c, a, slot, len) + STEP - 1) / STEP;
+                lenv[r] = len <= 0 ? 0u : (uint32_t)len > a.max_len ? a.max_len | 0x80000000u : (uint32_t)len;
+                slotv[r] = (uint32_t)slot;
+            }
+            sum += n[i];
         }
-        uint32_t sum = s;
+        uint32_t at = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= (uint32_t)o) sum += u;
+            const uint32_t u = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= (uint32_t)o) at += u;
         }
-        if (lane == 31) info[warp] = sum;
+        uint32_t *ws = (uint32_t *)(smem + X::INFO);
+        if (lane == 31) ws[warp] = at;
         __syncthreads();
-        uint32_t at = sum - s;
-        for (uint32_t w = 0; w < warp; w++) at += info[w];
+        at -= sum;
+        for (uint32_t w = 0; w < warp; w++) at += ws[w];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (tid * 4 + i <= a.nb) first[tid * 4 + i] = at;
+        for (int i = 0; i < 8; i++) {
+            if (tid * 8 + i < a.nb) first[tid * 8 + i] = at;
             at += n[i];
+            if (tid * 8 + i + 1 == a.nb) first[a.nb] = at;
         }
-        if (tid == 255 && a.nb == KV8_MAX_ROWS) first[KV8_MAX_ROWS] = at;
         __syncthreads();
     }
-    const uint32_t tasks = first[a.nb] * c.kvh;
-    const uint32_t lo = (uint32_t)((uint64_t)blockIdx.x * tasks / gridDim.x), hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * tasks / gridDim.x);
     for (uint32_t r = blockIdx.x; r < a.nb; r += gridDim.x)  // rows of length 0
-        if (first[r] == first[r + 1] && a.slots[r] >= 0)
-            for (uint32_t i = tid; i < a.qh * HD; i += 256) ((T *)a.y)[(int64_t)r * a.y_row + (int64_t)(i / HD) * a.y_head + i % HD] = kv8_round<T>(0.f);
-    if (lo >= hi) return;
+        if (first[r] == first[r + 1] && (int)slotv[r] >= 0)
+            for (uint32_t i = tid; i < a.qh * HD; i += 128) ((T *)a.y)[(int64_t)r * a.y_row + (int64_t)(i / HD) * a.y_head + i % HD] = kv8_round<T>(0.f);
+    const uint32_t total = first[a.nb] * c.kvh, W = gridDim.x * 4, w0 = warp * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
+    const uint32_t lo = (uint32_t)((uint64_t)w0 * total / W), hi = (uint32_t)((uint64_t)(w0 + 1) * total / W);
 
-    struct Task {
-        uint32_t r, h, ch, nch, tiles, n;  // n: tokens (of entries) from the chunk's start
-        int slot, len;
+    // ---- the feeding side: the task whose tiles are fetched next
+    uint32_t fr = 0, fh = 0, fch = 0, fat = 0;          // row, kv head, chunk; the task's first step
+    uint32_t fsteps = 0, fcs = 0, flen = 0, fn = 0;     // of the row: steps, steps of a chunk, length, tokens (of entries)
+    int fslot = 0;
+    auto row_of = [&]() {
+        fsteps = first[fr + 1] - first[fr];
+        flen = lenv[fr] & 0x7fffffffu;
+        fslot = (int)slotv[fr];
+        fn = row_tokens(c, a, fslot, (int)flen);
+        fcs = chunk_of(fn) / STEP;
     };
-    auto task_of = [&](uint32_t i) {
-        Task k;
-        const uint32_t x = i / c.kvh;
-        uint32_t l = 0, u = a.nb;  // the last row with first[row] <= x
+    auto settle = [&]() {  // after fch or fh may have run over
+        if (fch * fcs >= fsteps) fch = 0, fh++;
+        if (fh >= c.kvh) {
+            fh = 0;
+            do fr++;
+            while (fr < a.nb && first[fr + 1] == first[fr]);
+            if (fr < a.nb) row_of();
+        }
+        fat = fr < a.nb ? first[fr] * c.kvh + fh * fsteps + fch * fcs : total;
+    };
+    if (lo < hi) {
+        uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
         while (u - l > 1) {
             const uint32_t m = (l + u) >> 1;
-            if (first[m] <= x) l = m;
+            if (first[m] * c.kvh <= lo) l = m;
             else u = m;
         }
-        k.r = l;
-        k.nch = first[l + 1] - first[l];
-        const uint32_t rem = i - first[l] * c.kvh;
-        k.h = rem / k.nch;
-        k.ch = rem - k.h * k.nch;
-        k.slot = a.slots[l];
-        k.len = (int)min((uint32_t)a.lens[l], a.max_len);
-        k.n = min(CHUNK, row_tokens(c, a, l) - k.ch * CHUNK);
-        k.tiles = (k.n + TOK - 1) / TOK;
-        return k;
-    };
-
-    // ---- loads: lane i of warp 0 looks up and fetches rows i * box_rows .. of a tile
-    uint32_t fi = lo, ftile = 0;  // the next tile to look up
-    Task ft = task_of(lo);
-    uint32_t frow = 0, finfo = 0;  // of the tile looked up: number of the first row; valid tokens | 0x10000 (not in the cache)
-    bool fmore = true;             // a tile has been looked up and not fetched
-    auto look_up = [&]() {
-        frow = finfo = 0;
-        fmore = fi < hi;
-        if (!fmore) return;
-        const uint32_t o = ftile * TOK + lane * box_rows;
-        if (lane * box_rows < (uint32_t)TOK && o < ft.n) {
-            int64_t tok = ft.ch * CHUNK + o;
-            bool bad = false;
-            if (a.blocks) {
-                const uint32_t e = (uint32_t)tok / c.block;
-                const int b = e < a.nblocks ? __ldcg(a.blocks + ((size_t)ft.r * c.kvh + ft.h) * a.nblocks + e) : -1;
-                bad = b >= 0 && (uint32_t)b >= ((uint32_t)ft.len + c.block - 1) / c.block;
-                tok = b < 0 || bad ? ft.len : (int64_t)b * c.block + (uint32_t)tok % c.block;
+        fr = l;
+        row_of();
+        const uint32_t rem = lo - first[fr] * c.kvh;
+        fh = rem / fsteps;
+        fch = (rem - fh * fsteps + fcs - 1) / fcs;
+        settle();
+    } else fat = total;
+    // lane i < 16 has 16 tokens of the task: the number of their first row, how many there are | 0x10000: not in the cache
+    uint32_t grow = 0, gin = 0, gtok = 0;
+    int gpage = -1;
+    auto look_up = [&]() {  // asks for the page of every 16 tokens
+        gin = 0;
+        const uint32_t o = fch * fcs * STEP + lane * 16;
+        if (lane * 16 >= fcs * STEP || o >= fn) return;
+        int64_t tok = o;
+        if (a.blocks) {
+            const uint32_t e = o / c.block;
+            const int b = e < a.nblocks ? __ldcg(a.blocks + ((size_t)fr * c.kvh + fh) * a.nblocks + e) : -1;
+            if (b < 0) return;
+            if ((uint32_t)b >= (flen + c.block - 1) / c.block) {
+                gin = 16 | 0x10000u;
+                return;
             }
-            if (tok < ft.len) {
-                finfo = min(box_rows, (uint32_t)(ft.len - tok));
-                const int page = kv8_page(c, ft.slot, (int)(tok / KV8_PAGE));
-                if (page < 0) bad = true;
-                else frow = kv8_row0(c, page, 0, ft.h) + (uint32_t)tok % KV8_PAGE;
-            }
-            if (bad) finfo = box_rows | 0x10000u;
+            tok = (int64_t)b * c.block + o % c.block;
         }
-        if (++ftile == ft.tiles) {
-            ftile = 0;
-            if (++fi < hi) ft = task_of(fi);
-        }
+        if (tok >= flen) return;
+        gin = min(16u, (uint32_t)(flen - tok));
+        gtok = (uint32_t)tok;
+        gpage = kv8_entry_ok(c, fslot, gtok / KV8_PAGE) ? __ldcg(c.ptab + (size_t)fslot * c.max_pages + gtok / KV8_PAGE) : -1;
     };
-    auto fetch = [&](uint32_t j) {  // tile number j of the block: K into slot 2 j mod 3, V into the next
-        if (!fmore) return;
-        const uint32_t ks = 2 * j % 3, vs = (2 * j + 1) % 3;
-        if (lane < 16) info[lane] = finfo;
-        if (finfo >> 16) set_status(c.status, ST_BAD_ARG | 0x23);
-        const bool mine = finfo && !(finfo >> 16);
-        const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine)) * box_rows;
-        fence_proxy_async();  // the block's reads of the slots (ordered by the barrier) before the copies' writes
-        __syncwarp();
+    uint32_t fstep = 0, fed = 0;
+    auto feed_k = [&]() {  // tile number `fed`
+        if (fat >= hi) return;
+        if (fstep == 0) {  // the answers
+            if (gin && !(gin >> 16)) {
+                if (kv8_page_ok(c, gpage)) grow = kv8_row0(c, (uint32_t)gpage, 0, fh) + gtok % KV8_PAGE;
+                else gin |= 0x10000u;
+            }
+            if (gin >> 16) set_status(c.status, ST_BAD_ARG | 0x23);
+        }
+        const uint32_t sl = fed % RING, in0 = __shfl_sync(0xffffffffu, gin, 2 * fstep), in1 = __shfl_sync(0xffffffffu, gin, 2 * fstep + 1);
+        const uint32_t row0 = __shfl_sync(0xffffffffu, grow, 2 * fstep), row1 = __shfl_sync(0xffffffffu, grow, 2 * fstep + 1);
+        const uint32_t steps = min(fcs, fsteps - fch * fcs);
         if (lane == 0) {
-            mbar_expect_tx(&full[ks], n * (HD + 8));
-            mbar_expect_tx(&full[vs], n * HD);
+            info[2 * sl] = make_uint4(in0, in1, row0, row1);
+            info[2 * sl + 1] = make_uint4(fr, fh, fch, (fstep == 0 ? 1u : 0u) | (fstep + 1 == steps ? 2u : 0u));
+            const uint32_t on0 = in0 && !(in0 >> 16), on1 = box_rows == 16 && in1 && !(in1 >> 16);
+            fence_proxy_async();  // the warp's reads of the tile (ordered by __syncwarp) before the copies' writes
+            mbar_expect_tx(&kbar[sl], (on0 + on1) * box_rows * (HD + 8));
+            for (uint32_t e = 0; e < 2; e++)
+                if (e ? on1 : on0) {
+                    const uint32_t row = e ? row1 : row0;
+                    float *sc = scales + sl * 2 * STEP + e * 16;
+                    bulk_g2s(sc, c.scales + row, box_rows * 4, &kbar[sl]);
+                    bulk_g2s(sc + STEP, c.scales + row + c.kvh * KV8_PAGE, box_rows * 4, &kbar[sl]);
+#pragma unroll
+                    for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kb + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row, &kbar[sl]);
+                }
+        }
+        fed++;
+        if (++fstep == steps) {
+            fstep = 0;
+            fch++;
+            settle();
+            if (fat < hi) look_up();
         }
         __syncwarp();
-        if (mine) {
-            const uint32_t row = lane * box_rows, vrow = frow + c.kvh * KV8_PAGE;
-            float *sc = (float *)(smem + X::SCALES) + ks * 2 * TOK + row;
-            bulk_g2s(sc, c.scales + frow, box_rows * 4, &full[ks]);
-            bulk_g2s(sc + TOK, c.scales + vrow, box_rows * 4, &full[ks]);
-#pragma unroll
-            for (int d = 0; d < X::HALVES; d++) tma_load_2d(base + ks * X::SLOT + d * TOK * 128 + row * X::BOX, &tm, d * 128, (int)frow, &full[ks]);
-#pragma unroll
-            for (int d = 0; d < X::HALVES; d++) tma_load_2d(base + vs * X::SLOT + d * TOK * 128 + row * X::BOX, &tm, d * 128, (int)vrow, &full[vs]);
-        }
     };
-    if (warp == 0) {
-        look_up();
-        fetch(0);
-        look_up();
+    auto feed_v = [&](uint32_t n) {  // the V tile that belongs to K tile number n
+        if (n >= fed || lane) return;
+        const uint32_t sl = n % RING;
+        const uint4 f = info[2 * sl];
+        const uint32_t on0 = f.x && !(f.x >> 16), on1 = box_rows == 16 && f.y && !(f.y >> 16);
+        fence_proxy_async();
+        mbar_expect_tx(&vbar[sl], (on0 + on1) * box_rows * HD);
+        for (uint32_t e = 0; e < 2; e++)
+            if (e ? on1 : on0) {
+                const uint32_t row = (e ? f.w : f.z) + c.kvh * KV8_PAGE;
+#pragma unroll
+                for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vb + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row, &vbar[sl]);
+            }
+    };
+    if (fat < hi) look_up();
+    for (int i = 0; i < RING; i++) {
+        feed_k();
+        feed_v(i);
     }
 
-    bool dead = false, stop = false;  // this thread has given up a wait; some thread of the block has
-    uint32_t j = 0;                   // tiles done
+    // ---- the computing side
+    bool ok = true;
+    uint32_t n = 0, have_r = 0xffffffffu, have_h = 0;
     uint32_t qf[NT][HD / 8];
-    float fac[NT][2];
-    uint32_t have_r = 0xffffffffu, have_h = 0;
-    const uint32_t dg = warp % X::DG, tg = warp / X::DG;
-    for (uint32_t i = lo; i < hi; i++) {
-        const Task k = task_of(i);
-        if (k.r != have_r || k.h != have_h) {
-            // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
-            have_r = k.r, have_h = k.h;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const uint32_t head = nt * 8 + g;
-                const T *qp = (const T *)a.q + (int64_t)k.r * a.q_row + (int64_t)(k.h * a.G + min(head, a.G - 1)) * a.q_head;
-                uint32_t m = 0;
-#pragma unroll
-                for (int cc = 0; cc < HD / 64; cc++) {
-                    const int d0 = HD == 64 ? 16 * t : 128 * (cc >> 1) + 16 * (2 * t + (cc & 1));
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        uint32_t w[4];
-                        kv8_load_raw8(qp + d0 + 8 * e, w);
-#pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            qf[nt][cc * 8 + e * 4 + x] = w[x];
-                            const float2 f = kv8_float2<T>(w[x]);
-                            m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-                        }
-                    }
-                }
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const uint32_t ex = min(max(m >> 23, 1u), 253u);
-                const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
-#pragma unroll
-                for (int x = 0; x < HD / 8; x++) {
-                    const float2 f = kv8_float2<T>(qf[nt][x]);
-                    const __half2 h2 = __floats2half2_rn(f.x * down, f.y * down);
-                    qf[nt][x] = head < a.G ? *(const uint32_t *)&h2 : 0u;
-                }
-                const float f = up * (a.scale2 * kv8_unit<FMT>());
-                fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
-                fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-            }
-        }
-        float o[2][NT][4], m[NT][2], M[NT][2], l[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int x = 0; x < 4; x++) o[0][nt][x] = o[1][nt][x] = 0.f;
-            m[nt][0] = m[nt][1] = M[nt][0] = M[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
-        }
-        for (uint32_t tile = 0; tile < k.tiles; tile++, j++) {
-            const uint32_t ks = 2 * j % 3, vs = (2 * j + 1) % 3;
-            if (!dead && !mbar_wait(&full[ks], 2 * j / 3 & 1)) dead = true;
-            // ---- scores
-            float s[MT][NT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const uint32_t tok0 = (warp * MT + mt) * 16;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
-#pragma unroll
-                for (int cc = 0; cc < HD / 64; cc++) {
-                    const uint32_t ad = base + ks * X::SLOT + (HD == 64 ? (tok0 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4) : (cc >> 1) * TOK * 128 + (tok0 + g) * 128 + (((2 * t + (cc & 1)) ^ g) << 4));
-                    uint32_t v[4], u[4];
-                    lds128(v, ad);
-                    lds128(u, ad + 8 * X::BOX);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        uint32_t af[4];
-                        kv8_halves<FMT>(v[x], af[0], af[2]);
-                        kv8_halves<FMT>(u[x], af[1], af[3]);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_f16(s[mt][nt], af, qf[nt][cc * 8 + 2 * x], qf[nt][cc * 8 + 2 * x + 1], s[mt][nt]);
-                    }
-                }
-            }
-            float lv[MT][2];
-            float x0[NT][2], x1[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) x0[nt][0] = x0[nt][1] = x1[nt][0] = x1[nt][1] = -INFINITY;
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const uint32_t tok0 = (warp * MT + mt) * 16, inf = info[tok0 / box_rows], off = tok0 % box_rows;
-                const float *sc = (const float *)(smem + X::SCALES) + ks * 2 * TOK + tok0;
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t row = g + 8 * e;
-                    const bool in = off + row < (inf & 0xffffu), bad = inf >> 16;
-                    const float kscale = sc[row];
-                    lv[mt][e] = log2f(sc[TOK + row]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int d = 0; d < 2; d++) {
-                            float &v = s[mt][nt][2 * e + d];
-                            v = bad ? __uint_as_float(0x7fffffffu) : in ? v * (kscale * fac[nt][d]) : -INFINITY;
-                            x0[nt][d] = fmaxf(x0[nt][d], v);
-                            if (in && !bad) x1[nt][d] = fmaxf(x1[nt][d], v + lv[mt][e]);
-                        }
-                    if (!in || bad) lv[mt][e] = -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int d = 0; d < 2; d++)
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        x0[nt][d] = fmaxf(x0[nt][d], __shfl_xor_sync(0xffffffffu, x0[nt][d], off));
-                        x1[nt][d] = fmaxf(x1[nt][d], __shfl_xor_sync(0xffffffffu, x1[nt][d], off));
-                    }
-            if (g == 0) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) *(float4 *)(wmax + ((warp * NT + nt) * 4 + t) * 4) = make_float4(x0[nt][0], x1[nt][0], x0[nt][1], x1[nt][1]);
-            }
-            if ((stop = __syncthreads_or(dead))) break;
-            if (warp == 0) {
-                fetch(j + 1);
-                look_up();
-            }
-            // ---- weights
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float nm[2] = {m[nt][0], m[nt][1]}, nM[2] = {M[nt][0], M[nt][1]};
-#pragma unroll
-                for (int w = 0; w < 8; w++) {
-                    const float4 v = *(const float4 *)(wmax + ((w * NT + nt) * 4 + t) * 4);
-                    nm[0] = fmaxf(nm[0], v.x), nM[0] = fmaxf(nM[0], v.y);
-                    nm[1] = fmaxf(nm[1], v.z), nM[1] = fmaxf(nM[1], v.w);
-                }
-#pragma unroll
-                for (int d = 0; d < 2; d++) {
-                    l[nt][d] *= m[nt][d] == -INFINITY ? 0.f : exp2f(m[nt][d] - nm[d]);
-                    const float f = M[nt][d] == -INFINITY ? 0.f : exp2f(M[nt][d] - nM[d]);
-#pragma unroll
-                    for (int x = 0; x < 2; x++) o[x][nt][d] *= f, o[x][nt][2 + d] *= f;
-                    m[nt][d] = nm[d], M[nt][d] = nM[d];
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    uint32_t w[4];  // [token g, g + 8][head 2t, 2t + 1]: high part | remainder << 16
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-#pragma unroll
-                        for (int d = 0; d < 2; d++) {
-                            const float v = s[mt][nt][2 * e + d], sv = v + lv[mt][e];
-                            l[nt][d] += v == -INFINITY ? 0.f : exp2f(v - nm[d]);
-                            const float wt = sv == -INFINITY ? 0.f : exp2f(sv - nM[d]);
-                            const __half h = __float2half_rn(wt), r = __float2half_rn(wt - __half2float(h));
-                            w[2 * e + d] = (uint32_t)__half_as_ushort(h) | (uint32_t)__half_as_ushort(r) << 16;
-                        }
-                    // lanes of tokens g, g ^ 1 swap: the even one writes both tokens of head 2t, the odd one those of head 2t + 1
-                    const bool odd = g & 1;
-                    const uint32_t p0 = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 4), p1 = __shfl_xor_sync(0xffffffffu, odd ? w[2] : w[3], 4);
-                    const uint32_t a0 = odd ? p0 : w[0], b0 = odd ? w[1] : p0, a1 = odd ? p1 : w[2], b1 = odd ? w[3] : p1;
-                    *(uint4 *)(smem + X::P + (((warp * MT + mt) * NT + nt) * 8 + 2 * t + odd) * 64 + (g >> 1) * 16) =
-                        make_uint4(__byte_perm(a0, b0, 0x5410), __byte_perm(a1, b1, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x7632));
-                }
-            }
-            __syncthreads();
-            if (!dead && !mbar_wait(&full[vs], (2 * j + 1) / 3 & 1)) dead = true;
-            // ---- values
-            const uint32_t tv = base + vs * X::SLOT + (HD == 64 ? 2 * t * 64 + (((dg * 2 + (g >> 2)) ^ t) << 4) : (dg >> 2) * TOK * 128 + 2 * t * 128 + ((((dg & 3) * 2 + (g >> 2)) ^ (2 * t)) << 4)) + (g & 3) * 4;
-            const uint32_t tv1 = HD == 64 ? tv + 64 : (tv ^ 16) + 128;  // the next token: its row, and its swizzle
-#pragma unroll 4
-            for (int q = 0; q < X::KS; q++) {
-                const uint32_t st = tg * X::KS + q, ro = st * 16 * X::BOX;
-                const uint32_t wa = lds32(tv + ro), wb = lds32(tv1 + ro), wc = lds32(tv + ro + 8 * X::BOX), wd = lds32(tv1 + ro + 8 * X::BOX);
-                uint32_t a0[4], a1[4];  // channels 4g, 4g + 1 and 4g + 2, 4g + 3
-                kv8_halves<FMT>(__byte_perm(wa, wb, 0x5140), a0[0], a0[1]);
-                kv8_halves<FMT>(__byte_perm(wc, wd, 0x5140), a0[2], a0[3]);
-                kv8_halves<FMT>(__byte_perm(wa, wb, 0x7362), a1[0], a1[1]);
-                kv8_halves<FMT>(__byte_perm(wc, wd, 0x7362), a1[2], a1[3]);
+    float fac[NT][2], o[X::CH][NT][4], M[NT][2], l[NT][2];
+    for (; n < fed; n++) {
+        const uint32_t sl = n % RING;
+        const uint4 in = info[2 * sl], task = info[2 * sl + 1];
+        if (task.w & 1) {
+            if (task.x != have_r || task.y != have_h) {
+                // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
+                have_r = task.x, have_h = task.y;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    uint32_t p[4];
-                    lds128(p, base + X::P + (st * NT + nt) * 512 + lane * 16);
-                    mma_f16(o[0][nt], a0, p[0], p[1], o[0][nt]);
-                    mma_f16(o[1][nt], a1, p[0], p[1], o[1][nt]);
-                    mma_f16(o[0][nt], a0, p[2], p[3], o[0][nt]);
-                    mma_f16(o[1][nt], a1, p[2], p[3], o[1][nt]);
+                    const uint32_t head = nt * 8 + g;
+                    const T *qp = (const T *)a.q + (int64_t)task.x * a.q_row + (int64_t)(task.y * a.G + min(head, a.G - 1)) * a.q_head;
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int cc = 0; cc < HD / 64; cc++) {
+                        const int d0 = HD == 64 ? 16 * t : 128 * (cc >> 1) + 16 * (2 * t + (cc & 1));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            uint32_t w[4];
+                            kv8_load_raw8(qp + d0 + 8 * e, w);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                qf[nt][cc * 8 + e * 4 + x] = w[x];
+                                const float2 f = kv8_float2<T>(w[x]);
+                                m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                            }
+                        }
+                    }
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const uint32_t ex = min(max(m >> 23, 1u), 253u);
+                    const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+#pragma unroll
+                    for (int x = 0; x < HD / 8; x++) {
+                        const float2 f = kv8_float2<T>(qf[nt][x]);
+                        const __half2 h2 = __floats2half2_rn(f.x * down, f.y * down);
+                        qf[nt][x] = head < a.G ? *(const uint32_t *)&h2 : 0u;
+                    }
+                    const float f = up * a.scale2;
+                    fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+                    fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
                 }
             }
-        }
-        if (stop) break;
-        // ---- the chunk's totals
-        float *ex = (float *)(smem + X::P);  // sums over the tokens of other warps, [tg - 1][dg][NT][8 heads][32 channels], where the weights were
-        if (X::TG > 1 && (stop = __syncthreads_or(dead))) break;
-        if (X::TG > 1 && tg > 0) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                for (int d = 0; d < 2; d++)
-                    *(float4 *)(ex + (((((tg - 1) * X::DG + dg) * NT + nt) * 8 + 2 * t + d) * 8 + g) * 4) = make_float4(o[0][nt][d], o[0][nt][2 + d], o[1][nt][d], o[1][nt][2 + d]);
+                for (int x = 0; x < X::CH; x++) o[x][nt][0] = o[x][nt][1] = o[x][nt][2] = o[x][nt][3] = 0.f;
+                M[nt][0] = M[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.f;
+            }
         }
+        if (!mbar_wait(&kbar[sl], n / RING & 1)) {
+            ok = false;
+            break;
+        }
+        // ---- scores
+        float s[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < HD / 64; cc++)
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const uint32_t ad = Kb + sl * X::TILE + (HD == 64 ? (mt * 16 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4) : (cc >> 1) * STEP * 128 + (mt * 16 + g) * 128 + (((2 * t + (cc & 1)) ^ g) << 4));
+                uint32_t v[4], u[4];
+                lds128(v, ad);
+                lds128(u, ad + 8 * X::BOX);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    uint32_t af[4];
+                    kv8_operands<FMT>(v[x], af[0], af[2]);
+                    kv8_operands<FMT>(u[x], af[1], af[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma_f16(s[mt][nt], af, qf[nt][cc * 8 + 2 * x], qf[nt][cc * 8 + 2 * x + 1], s[mt][nt]);
+                }
+            }
+        float ks[2][2], lv[2][2], x1[NT][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float *sc = scales + sl * 2 * STEP + mt * 16 + g + 8 * e;
+                ks[mt][e] = sc[0], lv[mt][e] = sc[STEP];
+            }
+        __syncwarp();
+        feed_k();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) x1[nt][0] = x1[nt][1] = -INFINITY;
+        const uint32_t cnt[2] = {in.x >> 16 ? 0u : in.x, in.y >> 16 ? 0u : in.y};  // valid tokens of either 16
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+            const bool bad = (mt ? in.y : in.x) >> 16;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool have = g + 8 * e < cnt[mt];
+                const float vscale = lv[mt][e];
+                const bool nan = bad || (have && vscale != vscale);  // (a key's scale that is no number makes the score one by itself)
+                // a scale below 2^-110, which put does not make, counts as 2^-110 here
+                lv[mt][e] = !have ? -INFINITY : vscale < LOWEST ? LOWEST_LOG2 : __log2f(vscale);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        float &v = s[mt][nt][2 * e + d];
+                        v = nan ? __uint_as_float(0x7fffffffu) : have ? v * (ks[mt][e] * fac[nt][d]) : -INFINITY;
+                        if (have) x1[nt][d] = fmaxf(x1[nt][d], v + lv[mt][e]);
+                    }
+            }
+        }
+        bool up = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
 #pragma unroll
-                for (int off = 4; off < 32; off <<= 1) l[nt][d] += __shfl_xor_sync(0xffffffffu, l[nt][d], off);
-                if (g == 0) lsum[warp * NT * 8 + nt * 8 + 2 * t + d] = l[nt][d];
+                for (int off = 4; off < 32; off <<= 1) x1[nt][d] = fmaxf(x1[nt][d], __shfl_xor_sync(0xffffffffu, x1[nt][d], off));
+                up |= x1[nt][d] > M[nt][d];
             }
-        if ((stop = __syncthreads_or(dead))) break;
-        if (tg == 0) {
-            const bool poison = a.lens[k.r] > 0 && (uint32_t)a.lens[k.r] > a.max_len;
-            if (poison && tid == 0) set_status(c.status, ST_BAD_ARG | 0x24);
+        if (__any_sync(0xffffffffu, up)) {  // a larger maximum
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int d = 0; d < 2; d++) {
-                    const uint32_t head = nt * 8 + 2 * t + d;
-                    if (head >= a.G) continue;
-                    float4 v = make_float4(o[0][nt][d], o[0][nt][2 + d], o[1][nt][d], o[1][nt][2 + d]);
+                    const float nm = fmaxf(M[nt][d], x1[nt][d]), f = M[nt][d] == -INFINITY ? 0.f : exp2_fast(M[nt][d] - nm);
+                    M[nt][d] = nm;
+                    l[nt][d] *= f;
 #pragma unroll
-                    for (int x = 1; x < X::TG; x++) {
-                        const float4 u = *(const float4 *)(ex + (((((x - 1) * X::DG + dg) * NT + nt) * 8 + 2 * t + d) * 8 + g) * 4);
-                        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-                    }
-                    float lt = lsum[head];
-#pragma unroll
-                    for (int w = 1; w < 8; w++) lt += lsum[w * NT * 8 + head];
-                    const uint32_t qh = k.h * a.G + head, ch0 = 32 * dg + 4 * g;
-                    constexpr float unit = kv8_unit<FMT>();
-                    if (k.nch > 1) {
-                        *(float4 *)(a.part + (((size_t)k.r * a.max_chunks + k.ch) * a.qh + qh) * HD + ch0) = make_float4(v.x * unit, v.y * unit, v.z * unit, v.w * unit);
-                        if (dg == 0 && g == 0) stats_of(a, HD, k.r, qh)[k.ch] = make_float4(M[nt][d], m[nt][d], lt, 0.f);
-                    } else finish<T>(a, k.r, qh, ch0, v, poison || lt != lt ? __uint_as_float(0x7fffffffu) : M[nt][d] == -INFINITY ? 0.f : exp2f(M[nt][d] - m[nt][d]) * unit / lt);
+                    for (int x = 0; x < X::CH; x++) o[x][nt][d] *= f, o[x][nt][2 + d] *= f;
                 }
         }
-        // (the next task's first barrier stands between these reads of shared memory and its writes)
+        // ---- weights as B operands: [16 tokens][high parts of tokens 2t, 2t + 1, of 2t + 8, 2t + 9, then the remainders] of head g
+        uint32_t p[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float wt[4];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        const float v = s[mt][nt][2 * e + d], off = v - M[nt][d];
+                        const bool none = v == -INFINITY;
+                        l[nt][d] += none ? 0.f : exp2_fast(off);
+                        wt[2 * e + d] = none ? 0.f : exp2_fast(off + lv[mt][e]);
+                    }
+                const __half2 h01 = __floats2half2_rn(wt[0], wt[1]), h23 = __floats2half2_rn(wt[2], wt[3]);
+                const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
+                const __half2 r01 = __floats2half2_rn(wt[0] - f01.x, wt[1] - f01.y), r23 = __floats2half2_rn(wt[2] - f23.x, wt[3] - f23.y);
+                const int srcA = 8 * t + (g >> 1), srcB = srcA + 4;
+                const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+                auto to_b = [&](const __half2 &h) {
+                    const uint32_t x = *(const uint32_t *)&h;
+                    return __byte_perm(__shfl_sync(0xffffffffu, x, srcA), __shfl_sync(0xffffffffu, x, srcB), sel);
+                };
+                p[mt][nt][0] = to_b(h01), p[mt][nt][1] = to_b(h23), p[mt][nt][2] = to_b(r01), p[mt][nt][3] = to_b(r23);
+            }
+        if (!mbar_wait(&vbar[sl], n / RING & 1)) {
+            ok = false;
+            break;
+        }
+        // ---- values
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int hf = 0; hf < X::HALVES; hf++) {
+                uint32_t w[4][4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9: 16 channels from 16 g (HD = 64: 8 from 8 g)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t row = mt * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
+                    if (HD == 64) lds64(w[e][0], w[e][1], Vb + sl * X::TILE + row * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8);
+                    else lds128(w[e], Vb + sl * X::TILE + hf * STEP * 128 + row * 128 + ((g ^ (2 * t + (e & 1))) << 4));
+                }
+                if (cnt[mt] < 16) {  // rows behind the last token may hold anything, and 0 times a code that is no number would reach every head
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (2 * t + (e & 1) + (e >> 1) * 8 >= cnt[mt]) w[e][0] = w[e][1] = w[e][2] = w[e][3] = 0;
+                }
+#pragma unroll
+                for (int x = 0; x < X::LANE / 4; x++) {
+                    uint32_t a0[4], a1[4];  // channels 4x, 4x + 1 and 4x + 2, 4x + 3 of the lane
+                    kv8_operands<FMT>(__byte_perm(w[0][x], w[1][x], 0x5140), a0[0], a0[1]);
+                    kv8_operands<FMT>(__byte_perm(w[2][x], w[3][x], 0x5140), a0[2], a0[3]);
+                    kv8_operands<FMT>(__byte_perm(w[0][x], w[1][x], 0x7362), a1[0], a1[1]);
+                    kv8_operands<FMT>(__byte_perm(w[2][x], w[3][x], 0x7362), a1[2], a1[3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float(&y0)[4] = o[hf * 8 + 2 * x][nt], (&y1)[4] = o[hf * 8 + 2 * x + 1][nt];
+                        mma_f16(y0, a0, p[mt][nt][0], p[mt][nt][1], y0);
+                        mma_f16(y1, a1, p[mt][nt][0], p[mt][nt][1], y1);
+                        mma_f16(y0, a0, p[mt][nt][2], p[mt][nt][3], y0);
+                        mma_f16(y1, a1, p[mt][nt][2], p[mt][nt][3], y1);
+                    }
+                }
+            }
+        __syncwarp();
+        feed_v(n + RING);
+        if (task.w & 2) {  // ---- the chunk's totals
+            const uint32_t len = lenv[task.x];
+            const uint32_t nch = chunks_in(row_tokens(c, a, (int)slotv[task.x], (int)(len & 0x7fffffffu)));
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    float lt = l[nt][d];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, off);
+                    const uint32_t head = nt * 8 + 2 * t + d, qh = task.y * a.G + head;
+                    if (head >= a.G) continue;
+                    float *dst = a.part + (((size_t)task.x * a.max_chunks + task.z) * a.qh + qh) * HD;
+                    const float f = len >> 31 ? __uint_as_float(0x7fffffffu) : lt == 0.f ? 0.f : 1.f / lt;
+                    if (nch > 1 && g == 0) stats_of(a, HD, task.x, qh)[task.z] = make_float2(M[nt][d], lt);
+#pragma unroll
+                    for (int hf = 0; hf < X::HALVES; hf++)
+#pragma unroll
+                        for (int x = 0; x < X::LANE / 4; x++) {
+                            const float(&y0)[4] = o[hf * 8 + 2 * x][nt], (&y1)[4] = o[hf * 8 + 2 * x + 1][nt];
+                            const float4 v = make_float4(y0[d], y0[2 + d], y1[d], y1[2 + d]);
+                            const uint32_t ch = hf * 128 + X::LANE * g + 4 * x;
+                            if (nch > 1) *(float4 *)(dst + ch) = v;
+                            else finish<T>(a, task.x, qh, ch, v, f);
+                        }
+                }
+        }
     }
-    if (stop) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
-        if (tid == 0) {
-            set_status(status, ST_MBAR_TIMEOUT | 0x23);
-            for (uint32_t e = 2 * j; e < 2 * j + 4; e++) mbar_wait(&full[e % 3], e / 3 & 1);
+    if (!ok && lane == 0) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
+        set_status(status, ST_MBAR_TIMEOUT | 0x23);
+        for (uint32_t x = n; x < fed; x++) {
+            mbar_wait(&kbar[x % RING], x / RING & 1);
+            if (x < n + RING) mbar_wait(&vbar[x % RING], x / RING & 1);
         }
     }
 }
@@ -460,27 +502,23 @@ __global__ void __launch_bounds__(256, 2) kv8_attn_k(const __grid_constant__ CUt
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     __shared__ float4 accs[16][16];
-    __shared__ float wm[8][2], wl[8];
+    __shared__ float wm[8], wl[8];
     pdl_sync();
     const uint32_t qh = blockIdx.x / (HD / 64), ch = blockIdx.x % (HD / 64) * 64, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % 16, cg = tid / 16;
-    const uint32_t n = row_tokens(c, a, r), nch = (n + CHUNK - 1) / CHUNK;
+    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], a.lens[r]));
     if (nch < 2) return;  // written by the core
-    const float4 *st = stats_of(a, HD, r, qh);
-    float m = -INFINITY, M = -INFINITY;
-    for (uint32_t k = tid; k < nch; k += 256) {
-        const float4 s = __ldcg(st + k);
-        M = fmaxf(M, s.x);
-        m = fmaxf(m, s.y);
-    }
-    m = warp_max(m), M = warp_max(M);
-    if (lane == 0) wm[warp][0] = m, wm[warp][1] = M;
+    const float2 *st = stats_of(a, HD, r, qh);
+    float M = -INFINITY;
+    for (uint32_t k = tid; k < nch; k += 256) M = fmaxf(M, __ldcg(&st[k].x));
+    M = warp_max(M);
+    if (lane == 0) wm[warp] = M;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; w++) m = fmaxf(m, wm[w][0]), M = fmaxf(M, wm[w][1]);
+    for (int w = 0; w < 8; w++) M = fmaxf(M, wm[w]);
     float l = 0.f;
     for (uint32_t k = tid; k < nch; k += 256) {
-        const float4 s = __ldcg(st + k);
-        l += s.y == -INFINITY ? s.z : s.z * exp2f(s.y - m);  // (0, or NaN, where a chunk has no maximum)
+        const float2 s = __ldcg(st + k);
+        l += s.x == -INFINITY ? s.y : s.y * exp2f(s.x - M);  // (0, or NaN, where a chunk has no maximum)
     }
     l = warp_sum(l);
     if (lane == 0) wl[warp] = l;
@@ -505,7 +543,8 @@ __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
         acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
     }
     const bool bad = (uint32_t)a.lens[r] > a.max_len;
-    finish<T>(a, r, qh, ch + 4 * tid, acc, l != l || bad ? __uint_as_float(0x7fffffffu) : M == -INFINITY ? 0.f : exp2f(M - m) / l);
+    if (bad && tid == 0) set_status(c.status, ST_BAD_ARG | 0x24);
+    finish<T>(a, r, qh, ch + 4 * tid, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
 }
 
 // Which kernel: by the format, the type of rows, and whether 8 or 16 heads share a kv head.
@@ -514,35 +553,46 @@ typedef void (*merge_kernel)(Kv8Dev, AttnArgs);
 struct Launch {
     core_kernel core;
     merge_kernel merge;
-    int smem;
+    int smem, blocks;  // shared memory but for 12 bytes per row; blocks per SM
 };
+template <int HD, int FMT, class T, int NT, bool FEW>
+Launch launch_of() {
+    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::BLOCKS};
+}
 template <int HD, int FMT, class T>
-Launch launch_of(bool wide) {
-    return wide ? Launch{kv8_attn_k<HD, FMT, T, 2>, kv8_merge_k<HD, T>, Core<HD, 2>::BYTES} : Launch{kv8_attn_k<HD, FMT, T, 1>, kv8_merge_k<HD, T>, Core<HD, 1>::BYTES};
+Launch launch_of(bool wide, bool few) {
+    if (few) return wide ? launch_of<HD, FMT, T, 2, true>() : launch_of<HD, FMT, T, 1, true>();
+    return wide ? launch_of<HD, FMT, T, 2, false>() : launch_of<HD, FMT, T, 1, false>();
 }
 template <int HD>
-Launch launch_of(uint32_t format, uint32_t dtype, bool wide) {
-    if (format == QW_KV8_E4M3) return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_E4M3, __half>(wide) : launch_of<HD, QW_KV8_E4M3, __nv_bfloat16>(wide);
-    return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_INT8, __half>(wide) : launch_of<HD, QW_KV8_INT8, __nv_bfloat16>(wide);
+Launch launch_of(uint32_t format, uint32_t dtype, bool wide, bool few) {
+    if (format == QW_KV8_E4M3) return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_E4M3, __half>(wide, few) : launch_of<HD, QW_KV8_E4M3, __nv_bfloat16>(wide, few);
+    return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_INT8, __half>(wide, few) : launch_of<HD, QW_KV8_INT8, __nv_bfloat16>(wide, few);
 }
-Launch launch_of(uint32_t hd, uint32_t format, uint32_t dtype, bool wide) {
-    return hd == 64 ? launch_of<64>(format, dtype, wide) : hd == 128 ? launch_of<128>(format, dtype, wide) : launch_of<256>(format, dtype, wide);
+Launch launch_of(uint32_t hd, uint32_t format, uint32_t dtype, bool wide, bool few) {
+    return hd == 64 ? launch_of<64>(format, dtype, wide, few) : hd == 128 ? launch_of<128>(format, dtype, wide, few) : launch_of<256>(format, dtype, wide, few);
 }
 
 uint32_t chunks_of(const qw_kv8_cache *c, uint32_t max_len, uint32_t nblocks) {
     const uint64_t blocks = ((uint64_t)max_len + c->block - 1) / c->block;
     const uint64_t n = nblocks ? (nblocks < blocks ? nblocks : blocks) * c->block : max_len;
-    return (uint32_t)((n + CHUNK - 1) / CHUNK);
+    // the most chunks of a row of up to n tokens: a longer row may have fewer, at the steps of chunk_of
+    const uint32_t m = (uint32_t)(n < 0xffffff00u ? n : 0xffffff00u);
+    uint32_t most = chunks_in(m);
+    for (uint32_t e : {512u, 2048u, 8192u})
+        if (e < m && chunks_in(e) > most) most = chunks_in(e);
+    return most;
 }
 const char *check_shape(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_t max_len) {
     if (nb < 1 || nb > KV8_MAX_ROWS) return "a call has 1 to 1024 rows";
     if (qh < c->kvh || qh % c->kvh || qh / c->kvh > 16) return "1 to 16 query heads share a kv head";
     if (qh > 65535) return "too many query heads";
+    if ((double)nb * c->kvh * ((double)max_len / 32 + 1) > 2147483647.0) return "more tokens than one call takes";
     if (max_len < 1 || (uint64_t)max_len > (uint64_t)c->max_pages * KV8_PAGE) return "max_len is 1 to 256 max_pages";
     return nullptr;
 }
 size_t work_of(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_t max_len, uint32_t nblocks) {
-    return (size_t)nb * chunks_of(c, max_len, nblocks) * qh * (c->hd + 4) * 4;
+    return (size_t)nb * chunks_of(c, max_len, nblocks) * qh * (c->hd + 2) * 4;
 }
 // 0, or -1 / -2 with a message
 int check_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, const char **m) {
@@ -565,11 +615,13 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     if (!tmap_2d(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, c->codes, c->hd, rows, c->hd, c->hd < 128 ? c->hd : 128, box_rows,
                  c->hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
-    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G > 8);
-    cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, L.smem);
+    const uint64_t most = (uint64_t)a->nb * mc * c->kvh, sms = (uint64_t)kv8_sm_count();
+    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G > 8, most <= 4 * sms);
+    const int smem = L.smem + (int)a->nb * 12;
+    cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    const uint64_t most = (uint64_t)a->nb * mc * c->kvh, fit = 2 * (uint64_t)kv8_sm_count();
-    e = qw_launch(L.core, (uint32_t)(most < fit ? most : fit), 256, L.smem, st, tm, d, k, box_rows, status);
+    const uint64_t fit = L.blocks * sms;
+    e = qw_launch(L.core, (uint32_t)(most < fit ? most : fit), 128, smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess || mc < 2) return e;
     return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
 }

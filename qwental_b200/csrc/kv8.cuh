@@ -35,6 +35,19 @@ __device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t &h01, uint32_t &
         h23 = kv8_int8_half2(__byte_perm(w, 0x64646464u, 0x4342));
     }
 }
+// The same for products: their values as fp16 numbers; an e4m3 code that is no number becomes a NaN.  (Two conversions per four codes instead of eight
+// operations; as many cycles of the pipe each.)
+template <int FMT>
+__device__ __forceinline__ void kv8_operands(uint32_t w, uint32_t &h01, uint32_t &h23) {
+    if (FMT == QW_KV8_E4M3)
+        asm("{\n\t.reg .b16 l, h;\n\t"
+            "mov.b32 {l, h}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(h01), "=r"(h23)
+            : "r"(w));
+    else kv8_halves<FMT>(w, h01, h23);
+}
 template <int FMT>
 __device__ __forceinline__ void kv8_decode4(uint32_t w, float (&x)[4]) {
     uint32_t a, b;
@@ -110,6 +123,9 @@ __device__ __forceinline__ float2 kv8_float2<__nv_bfloat16>(uint32_t w) { return
 
 __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void lds64(uint32_t &a, uint32_t &b, uint32_t addr) {
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
