@@ -97,6 +97,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, unsigned parity) {
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, unsigned parity) {  // does not suspend the thread
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait: polls for at most about two seconds of wall time (the global nanosecond timer), then gives up
 // with false; the caller records ST_MBAR_TIMEOUT and leaves.
 __device__ __forceinline__ uint64_t global_ns() {

@@ -59,7 +59,8 @@ __device__ __forceinline__ void finish(const AttnArgs &a, uint32_t r, uint32_t q
 // ------------------------------------------------------------------------------------------------ core
 // Independent warps: the (row, kv head, chunk) tasks of the launch are numbered in this order, each with as many steps of 32 tokens as it has, and a warp
 // takes those that start within its share of all steps.  It owns a task completely -- queries, running maximum and the sums of all channels in registers --
-// and feeds itself through a ring of K and V tiles with an mbarrier each, so warps wait for nothing but their own copies and overlap one another.
+// and is fed through a ring of K and V tiles of its own, so warps wait for nothing but their copies and overlap one another.  One warp of the block
+// feeds the others, lane w the ring of warp w (feeding themselves cost the warps 2000 to 4000 cycles in a step of 6000).
 //   scores   S[16 tokens][8 heads] = codes[16][HD] . q^T     mma m16n8k16.  Which channel is which k of the product is free as long as both sides agree, so a
 //            lane takes 16 codes with one shared-memory load and they feed four products as they lie.
 //   values   O^T[16 channels][8 heads] += codes^T[16][16 tokens] . w^T     a lane takes 16 codes of four tokens; byte permutations pair the tokens; the weights
@@ -74,38 +75,40 @@ template <int HD, int NT, bool FEW>
 struct Core {
     static constexpr int BOX = HD < 128 ? HD : 128, HALVES = HD / BOX;  // bytes of a row in a copy, copies side by side
     static constexpr int TILE = STEP * HD;                              // K or V
+    // warps that compute: what shared memory and registers (for warps in fours, the feeding one among them) allow, one block per SM
+    static constexpr int WARPS = FEW ? 4 : HD == 256 ? (NT == 1 ? 11 : 7) : NT == 1 ? 12 : 11;
     static constexpr int RING = (FEW ? 3 : 1) * 256 / HD;               // tiles of either: 16 KB per warp, or 48
-    static constexpr int BLOCKS = FEW ? 1 : NT == 1 ? 3 : 2;            // per SM: what shared memory and registers allow
     static constexpr int CH = HALVES * (HD < 128 ? 4 : 8);              // 16-channel tiles
     static constexpr int LANE = HD < 128 ? 8 : 16;                      // channels of a lane in a row of a copy
-    // shared memory behind the tiles; then 12 bytes per row
-    static constexpr int SCALES = 4 * RING * 2 * TILE, INFO = SCALES + 4 * RING * 2 * STEP * 4, BARS = INFO + 4 * RING * 32, ROWS = BARS + 4 * RING * 16, BYTES = ROWS + 1024 + 16;
+    static constexpr int SLOTS = WARPS * RING, THREADS = 32 * (WARPS + 1);
+    // shared memory behind the tiles: scales of K and V, what a tile is, mbarriers (full and empty, K and V); then 12 bytes per row
+    static constexpr int SCALES = SLOTS * 2 * TILE, INFO = SCALES + SLOTS * 2 * STEP * 4, BARS = INFO + SLOTS * 32, HAS = BARS + SLOTS * 32, ROWS = HAS + 64, BYTES = ROWS + 1024 + 16;
+    static_assert(WARPS + 1 <= 16 && BYTES + 12 * KV8_MAX_ROWS <= 227 * 1024, "words of HAS, and what a block may have");
 };
 
 template <int HD, int FMT, class T, int NT, bool FEW>
-__global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
+__global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
     typedef Core<HD, NT, FEW> X;
     constexpr int RING = X::RING;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // swizzled copies need it
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t Kb = smem_u32(smem) + warp * RING * 2 * X::TILE, Vb = Kb + RING * X::TILE;
-    float *scales = (float *)(smem + X::SCALES) + warp * RING * 2 * STEP;
-    uint4 *info = (uint4 *)(smem + X::INFO) + warp * RING * 2;
-    uint64_t *kbar = (uint64_t *)(smem + X::BARS) + warp * RING * 2, *vbar = kbar + RING;
-    uint32_t *first = (uint32_t *)(smem + X::ROWS), *lenv = first + a.nb + 1, *slotv = lenv + a.nb;
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < 2 * RING; i++) mbar_init(&kbar[i], 1);
-        mbar_init_fence();
-    }
+    uint32_t *has = (uint32_t *)(smem + X::HAS), *first = (uint32_t *)(smem + X::ROWS), *lenv = first + a.nb + 1, *slotv = lenv + a.nb;
+    // of warp w: its K tiles, then its V tiles; full and empty barriers of both
+    auto tiles_of = [&](uint32_t w) { return smem_u32(smem) + w * RING * 2 * X::TILE; };
+    auto scales_of = [&](uint32_t w) { return (float *)(smem + X::SCALES) + w * RING * 2 * STEP; };
+    auto info_of = [&](uint32_t w) { return (uint4 *)(smem + X::INFO) + w * RING * 2; };
+    auto bars_of = [&](uint32_t w) { return (uint64_t *)(smem + X::BARS) + w * RING * 4; };
+    for (uint32_t i = tid; i < X::SLOTS * 4; i += X::THREADS) mbar_init((uint64_t *)(smem + X::BARS) + i, 1);
+    mbar_init_fence();
     pdl_sync();
     // ---- rows: steps of one kv head, running sum; length (top bit: longer than the call allows), slot
     {
-        uint32_t n[8], sum = 0;
+        constexpr uint32_t PER = (KV8_MAX_ROWS + X::THREADS - 1) / X::THREADS;
+        uint32_t n[PER], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t r = tid * 8 + i;
+        for (int i = 0; i < PER; i++) {
+            const uint32_t r = tid * PER + i;
             n[i] = 0;
             if (r < a.nb) {
                 const int len = a.lens[r], slot = a.slots[r];
@@ -121,149 +124,184 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
             const uint32_t u = __shfl_up_sync(0xffffffffu, at, o);
             if (lane >= (uint32_t)o) at += u;
         }
-        uint32_t *ws = (uint32_t *)(smem + X::INFO);
-        if (lane == 31) ws[warp] = at;
+        if (lane == 31) has[warp] = at;
         __syncthreads();
         at -= sum;
-        for (uint32_t w = 0; w < warp; w++) at += ws[w];
+        for (uint32_t w = 0; w < warp; w++) at += has[w];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (tid * 8 + i < a.nb) first[tid * 8 + i] = at;
+        for (int i = 0; i < PER; i++) {
+            if (tid * PER + i < a.nb) first[tid * PER + i] = at;
             at += n[i];
-            if (tid * 8 + i + 1 == a.nb) first[a.nb] = at;
+            if (tid * PER + i + 1 == a.nb) first[a.nb] = at;
         }
         __syncthreads();
     }
     for (uint32_t r = blockIdx.x; r < a.nb; r += gridDim.x)  // rows of length 0
         if (first[r] == first[r + 1] && (int)slotv[r] >= 0)
-            for (uint32_t i = tid; i < a.qh * HD; i += 128) ((T *)a.y)[(int64_t)r * a.y_row + (int64_t)(i / HD) * a.y_head + i % HD] = kv8_round<T>(0.f);
-    const uint32_t total = first[a.nb] * c.kvh, W = gridDim.x * 4, w0 = warp * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
-    const uint32_t lo = (uint32_t)((uint64_t)w0 * total / W), hi = (uint32_t)((uint64_t)(w0 + 1) * total / W);
+            for (uint32_t i = tid; i < a.qh * HD; i += X::THREADS) ((T *)a.y)[(int64_t)r * a.y_row + (int64_t)(i / HD) * a.y_head + i % HD] = kv8_round<T>(0.f);
 
-    // ---- the feeding side: the task whose tiles are fetched next
-    uint32_t fr = 0, fh = 0, fch = 0, fat = 0;          // row, kv head, chunk; the task's first step
-    uint32_t fsteps = 0, fcs = 0, flen = 0, fn = 0;     // of the row: steps, steps of a chunk, length, tokens (of entries)
-    int fslot = 0;
-    auto row_of = [&]() {
-        fsteps = first[fr + 1] - first[fr];
-        flen = lenv[fr] & 0x7fffffffu;
-        fslot = (int)slotv[fr];
-        fn = row_tokens(c, a, fslot, (int)flen);
-        fcs = chunk_of(fn) / STEP;
-    };
-    auto settle = [&]() {  // after fch or fh may have run over
-        if (fch * fcs >= fsteps) fch = 0, fh++;
-        if (fh >= c.kvh) {
-            fh = 0;
-            do fr++;
-            while (fr < a.nb && first[fr + 1] == first[fr]);
-            if (fr < a.nb) row_of();
-        }
-        fat = fr < a.nb ? first[fr] * c.kvh + fh * fsteps + fch * fcs : total;
-    };
-    if (lo < hi) {
-        uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
-        while (u - l > 1) {
-            const uint32_t m = (l + u) >> 1;
-            if (first[m] * c.kvh <= lo) l = m;
-            else u = m;
-        }
-        fr = l;
-        row_of();
-        const uint32_t rem = lo - first[fr] * c.kvh;
-        fh = rem / fsteps;
-        fch = (rem - fh * fsteps + fcs - 1) / fcs;
-        settle();
-    } else fat = total;
-    // lane i < 16 has 16 tokens of the task: the number of their first row, how many there are | 0x10000: not in the cache
-    uint32_t grow = 0, gin = 0, gtok = 0;
-    int gpage = -1;
-    auto look_up = [&]() {  // asks for the page of every 16 tokens
-        gin = 0;
-        const uint32_t o = fch * fcs * STEP + lane * 16;
-        if (lane * 16 >= fcs * STEP || o >= fn) return;
-        int64_t tok = o;
-        if (a.blocks) {
-            const uint32_t e = o / c.block;
-            const int b = e < a.nblocks ? __ldcg(a.blocks + ((size_t)fr * c.kvh + fh) * a.nblocks + e) : -1;
-            if (b < 0) return;
-            if ((uint32_t)b >= (flen + c.block - 1) / c.block) {
-                gin = 16 | 0x10000u;
-                return;
+    // ---- the feeding warp: lane w has the task whose tiles warp w gets next
+    if (warp == X::WARPS) {
+        const uint32_t total = first[a.nb] * c.kvh, W = gridDim.x * X::WARPS, w0 = lane * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
+        const uint32_t lo = lane < X::WARPS ? (uint32_t)((uint64_t)w0 * total / W) : total, hi = lane < X::WARPS ? (uint32_t)((uint64_t)(w0 + 1) * total / W) : total;
+        uint32_t fr = 0, fh = 0, fch = 0, fat = total;      // row, kv head, chunk; the task's first step
+        uint32_t fsteps = 0, fcs = 1, flen = 0, fn = 0;     // of the row: steps, steps of a chunk, length, tokens (of entries)
+        int fslot = 0;
+        auto row_of = [&]() {
+            fsteps = first[fr + 1] - first[fr];
+            flen = lenv[fr] & 0x7fffffffu;
+            fslot = (int)slotv[fr];
+            fn = row_tokens(c, a, fslot, (int)flen);
+            fcs = chunk_of(fn) / STEP;
+        };
+        auto settle = [&]() {  // after fch or fh may have run over
+            if (fch * fcs >= fsteps) fch = 0, fh++;
+            if (fh >= c.kvh) {
+                fh = 0;
+                do fr++;
+                while (fr < a.nb && first[fr + 1] == first[fr]);
+                if (fr < a.nb) row_of();
             }
-            tok = (int64_t)b * c.block + o % c.block;
-        }
-        if (tok >= flen) return;
-        gin = min(16u, (uint32_t)(flen - tok));
-        gtok = (uint32_t)tok;
-        gpage = kv8_entry_ok(c, fslot, gtok / KV8_PAGE) ? __ldcg(c.ptab + (size_t)fslot * c.max_pages + gtok / KV8_PAGE) : -1;
-    };
-    uint32_t fstep = 0, fed = 0;
-    auto feed_k = [&]() {  // tile number `fed`
-        if (fat >= hi) return;
-        if (fstep == 0) {  // the answers
-            if (gin && !(gin >> 16)) {
-                if (kv8_page_ok(c, gpage)) grow = kv8_row0(c, (uint32_t)gpage, 0, fh) + gtok % KV8_PAGE;
-                else gin |= 0x10000u;
+            fat = fr < a.nb ? first[fr] * c.kvh + fh * fsteps + fch * fcs : total;
+        };
+        if (lo < hi) {
+            uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
+            while (u - l > 1) {
+                const uint32_t m = (l + u) >> 1;
+                if (first[m] * c.kvh <= lo) l = m;
+                else u = m;
             }
-            if (gin >> 16) set_status(c.status, ST_BAD_ARG | 0x23);
-        }
-        const uint32_t sl = fed % RING, in0 = __shfl_sync(0xffffffffu, gin, 2 * fstep), in1 = __shfl_sync(0xffffffffu, gin, 2 * fstep + 1);
-        const uint32_t row0 = __shfl_sync(0xffffffffu, grow, 2 * fstep), row1 = __shfl_sync(0xffffffffu, grow, 2 * fstep + 1);
-        const uint32_t steps = min(fcs, fsteps - fch * fcs);
-        if (lane == 0) {
-            info[2 * sl] = make_uint4(in0, in1, row0, row1);
-            info[2 * sl + 1] = make_uint4(fr, fh, fch, (fstep == 0 ? 1u : 0u) | (fstep + 1 == steps ? 2u : 0u));
-            const uint32_t on0 = in0 && !(in0 >> 16), on1 = box_rows == 16 && in1 && !(in1 >> 16);
-            fence_proxy_async();  // the warp's reads of the tile (ordered by __syncwarp) before the copies' writes
-            mbar_expect_tx(&kbar[sl], (on0 + on1) * box_rows * (HD + 8));
-            for (uint32_t e = 0; e < 2; e++)
-                if (e ? on1 : on0) {
-                    const uint32_t row = e ? row1 : row0;
-                    float *sc = scales + sl * 2 * STEP + e * 16;
-                    bulk_g2s(sc, c.scales + row, box_rows * 4, &kbar[sl]);
-                    bulk_g2s(sc + STEP, c.scales + row + c.kvh * KV8_PAGE, box_rows * 4, &kbar[sl]);
-#pragma unroll
-                    for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kb + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row, &kbar[sl]);
-                }
-        }
-        fed++;
-        if (++fstep == steps) {
-            fstep = 0;
-            fch++;
+            fr = l;
+            row_of();
+            const uint32_t rem = lo - first[fr] * c.kvh;
+            fh = rem / fsteps;
+            fch = (rem - fh * fsteps + fcs - 1) / fcs;
             settle();
-            if (fat < hi) look_up();
         }
-        __syncwarp();
-    };
-    auto feed_v = [&](uint32_t n) {  // the V tile that belongs to K tile number n
-        if (n >= fed || lane) return;
-        const uint32_t sl = n % RING;
-        const uint4 f = info[2 * sl];
-        const uint32_t on0 = f.x && !(f.x >> 16), on1 = box_rows == 16 && f.y && !(f.y >> 16);
-        fence_proxy_async();
-        mbar_expect_tx(&vbar[sl], (on0 + on1) * box_rows * HD);
-        for (uint32_t e = 0; e < 2; e++)
-            if (e ? on1 : on0) {
-                const uint32_t row = (e ? f.w : f.z) + c.kvh * KV8_PAGE;
+        // a tile: 16 tokens each -- valid ones | 0x10000 (not in the cache), token and page of the first
+        uint32_t in[2], tok[2], fstep = 0;
+        int page[2];
+        auto ask = [&]() {
+            const uint32_t o = (fch * fcs + fstep) * STEP;
 #pragma unroll
-                for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vb + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row, &vbar[sl]);
+            for (int e = 0; e < 2; e++) {
+                in[e] = 0;
+                page[e] = -1;
+                uint32_t x = o + 16 * e;
+                if (x >= fn) continue;
+                if (a.blocks) {
+                    if (e && box_rows != 16) {  // the same block
+                        x = tok[0] + 16;
+                        if (!in[0] || in[0] >> 16) continue;
+                    } else {
+                        const uint32_t en = x / c.block;
+                        const int b = en < a.nblocks ? __ldcg(a.blocks + ((size_t)fr * c.kvh + fh) * a.nblocks + en) : -1;
+                        if (b < 0) continue;
+                        if ((uint32_t)b >= (flen + c.block - 1) / c.block) {
+                            in[e] = 16 | 0x10000u;
+                            continue;
+                        }
+                        x = (uint32_t)b * c.block + x % c.block;
+                    }
+                }
+                tok[e] = x;
+                if (x >= flen) continue;
+                in[e] = min(16u, flen - x);
+                if ((e == 0 || box_rows == 16) && kv8_entry_ok(c, fslot, x / KV8_PAGE)) page[e] = __ldcg(c.ptab + (size_t)fslot * c.max_pages + x / KV8_PAGE);
             }
-    };
-    if (fat < hi) look_up();
-    for (int i = 0; i < RING; i++) {
-        feed_k();
-        feed_v(i);
+        };
+        bool more = lane < X::WARPS && fat < hi;
+        if (lane < X::WARPS) has[lane] = more;
+        __syncthreads();
+        if (more) ask();
+        uint64_t *bars = bars_of(lane < X::WARPS ? lane : 0);
+        uint4 *info = info_of(lane < X::WARPS ? lane : 0);
+        float *scales = scales_of(lane < X::WARPS ? lane : 0);
+        const uint32_t Kt = tiles_of(lane < X::WARPS ? lane : 0), Vt = Kt + RING * X::TILE, vrows = c.kvh * KV8_PAGE;
+        uint32_t fed = 0, vfed = 0;  // K and V tiles so far
+        uint64_t t0 = global_ns();
+        bool ok = true;
+        while (__any_sync(0xffffffffu, more || vfed < fed)) {
+            bool did = false;
+            const uint32_t sl = fed % RING, vl = vfed % RING;
+            if (more && fed < vfed + RING /* V of the tile whose place it takes has gone */ && (fed < RING || mbar_test(&bars[2 * RING + sl], fed / RING - 1 & 1))) {
+                uint32_t row[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (in[e] && !(in[e] >> 16) && (e == 0 || box_rows == 16)) {
+                        if (kv8_page_ok(c, page[e])) row[e] = kv8_row0(c, (uint32_t)page[e], 0, fh) + tok[e] % KV8_PAGE;
+                        else in[e] |= 0x10000u;
+                    }
+                if (box_rows != 16 && in[0] >> 16 && in[1]) in[1] |= 0x10000u;
+                if ((in[0] | in[1]) >> 16) set_status(c.status, ST_BAD_ARG | 0x23);
+                const bool on0 = in[0] && !(in[0] >> 16), on1 = box_rows == 16 && in[1] && !(in[1] >> 16);
+                const uint32_t steps = min(fcs, fsteps - fch * fcs), of = (fstep == 0 ? 1u : 0u) | (fstep + 1 == steps ? 2u : 0u), r = fr, h = fh, ch = fch;
+                info[2 * sl] = make_uint4(in[0], in[1], row[0], row[1]);
+                if (++fstep == steps) {
+                    fstep = 0;
+                    fch++;
+                    settle();
+                    more = fat < hi;
+                }
+                info[2 * sl + 1] = make_uint4(r, h, ch, of | (more ? 0u : 4u));
+                mbar_expect_tx(&bars[sl], (on0 + on1) * box_rows * (HD + 8));
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (e ? on1 : on0) {
+                        float *sc = scales + sl * 2 * STEP + e * 16;
+#pragma unroll
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kt + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row[e], &bars[sl]);
+                        bulk_g2s(sc, c.scales + row[e], box_rows * 4, &bars[sl]);
+                        bulk_g2s(sc + STEP, c.scales + row[e] + vrows, box_rows * 4, &bars[sl]);
+                    }
+                fed++;
+                if (more) ask();
+                did = true;
+            }
+            if (vfed < fed && (vfed < RING || mbar_test(&bars[3 * RING + vl], vfed / RING - 1 & 1))) {
+                const uint4 f = info[2 * vl];
+                const bool on0 = f.x && !(f.x >> 16), on1 = box_rows == 16 && f.y && !(f.y >> 16);
+                mbar_expect_tx(&bars[RING + vl], (on0 + on1) * box_rows * HD);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (e ? on1 : on0) {
+#pragma unroll
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? f.w : f.z) + vrows), &bars[RING + vl]);
+                    }
+                vfed++;
+                did = true;
+            }
+            if (__any_sync(0xffffffffu, did)) t0 = global_ns();
+            else if (__any_sync(0xffffffffu, global_ns() - t0 > 2000000000ull)) {
+                ok = false;
+                break;
+            }
+        }
+        if (!ok) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
+            if (lane == 0) set_status(status, ST_MBAR_TIMEOUT | 0x23);
+            for (uint32_t x = fed < RING ? 0 : fed - RING; x < fed; x++) mbar_wait(&bars[x % RING], x / RING & 1);
+            for (uint32_t x = vfed < RING ? 0 : vfed - RING; x < vfed; x++) mbar_wait(&bars[RING + x % RING], x / RING & 1);
+        }
+        return;
     }
+    __syncthreads();
+    if (!has[warp]) return;
 
     // ---- the computing side
-    bool ok = true;
+    bool ok = true, more = true;
     uint32_t n = 0, have_r = 0xffffffffu, have_h = 0;
     uint32_t qf[NT][HD / 8];
     float fac[NT][2], o[X::CH][NT][4], M[NT][2], l[NT][2];
-    for (; n < fed; n++) {
+    const uint32_t Kb = tiles_of(warp), Vb = Kb + RING * X::TILE;
+    uint64_t *bars = bars_of(warp);
+    for (; more; n++) {
         const uint32_t sl = n % RING;
-        const uint4 in = info[2 * sl], task = info[2 * sl + 1];
+        if (!mbar_wait(&bars[sl], n / RING & 1)) {
+            ok = false;
+            break;
+        }
+        const uint4 in = info_of(warp)[2 * sl], task = info_of(warp)[2 * sl + 1];
+        more = !(task.w & 4);
         if (task.w & 1) {
             if (task.x != have_r || task.y != have_h) {
                 // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
@@ -311,10 +349,6 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
                 l[nt][0] = l[nt][1] = 0.f;
             }
         }
-        if (!mbar_wait(&kbar[sl], n / RING & 1)) {
-            ok = false;
-            break;
-        }
         // ---- scores
         float s[2][NT][4];
 #pragma unroll
@@ -343,11 +377,9 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float *sc = scales + sl * 2 * STEP + mt * 16 + g + 8 * e;
+                const float *sc = scales_of(warp) + sl * 2 * STEP + mt * 16 + g + 8 * e;
                 ks[mt][e] = sc[0], lv[mt][e] = sc[STEP];
             }
-        __syncwarp();
-        feed_k();
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) x1[nt][0] = x1[nt][1] = -INFINITY;
         const uint32_t cnt[2] = {in.x >> 16 ? 0u : in.x, in.y >> 16 ? 0u : in.y};  // valid tokens of either 16
@@ -380,6 +412,8 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
                 for (int off = 4; off < 32; off <<= 1) x1[nt][d] = fmaxf(x1[nt][d], __shfl_xor_sync(0xffffffffu, x1[nt][d], off));
                 up |= x1[nt][d] > M[nt][d];
             }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[2 * RING + sl]);
         if (__any_sync(0xffffffffu, up)) {  // a larger maximum
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -419,7 +453,7 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
                 };
                 p[mt][nt][0] = to_b(h01), p[mt][nt][1] = to_b(h23), p[mt][nt][2] = to_b(r01), p[mt][nt][3] = to_b(r23);
             }
-        if (!mbar_wait(&vbar[sl], n / RING & 1)) {
+        if (!mbar_wait(&bars[RING + sl], n / RING & 1)) {
             ok = false;
             break;
         }
@@ -458,7 +492,7 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
                 }
             }
         __syncwarp();
-        feed_v(n + RING);
+        if (lane == 0) mbar_arrive(&bars[3 * RING + sl]);
         if (task.w & 2) {  // ---- the chunk's totals
             const uint32_t len = lenv[task.x];
             const uint32_t nch = chunks_in(row_tokens(c, a, (int)slotv[task.x], (int)(len & 0x7fffffffu)));
@@ -487,13 +521,7 @@ __global__ void __launch_bounds__(128, Core<HD, NT, FEW>::BLOCKS) kv8_attn_k(con
                 }
         }
     }
-    if (!ok && lane == 0) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
-        set_status(status, ST_MBAR_TIMEOUT | 0x23);
-        for (uint32_t x = n; x < fed; x++) {
-            mbar_wait(&kbar[x % RING], x / RING & 1);
-            if (x < n + RING) mbar_wait(&vbar[x % RING], x / RING & 1);
-        }
-    }
+    if (!ok && lane == 0) set_status(status, ST_MBAR_TIMEOUT | 0x23);
 }
 
 // ------------------------------------------------------------------------------------------------ join
@@ -553,11 +581,11 @@ typedef void (*merge_kernel)(Kv8Dev, AttnArgs);
 struct Launch {
     core_kernel core;
     merge_kernel merge;
-    int smem, blocks;  // shared memory but for 12 bytes per row; blocks per SM
+    int smem, threads;  // shared memory but for 12 bytes per row
 };
 template <int HD, int FMT, class T, int NT, bool FEW>
 Launch launch_of() {
-    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::BLOCKS};
+    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::THREADS};
 }
 template <int HD, int FMT, class T>
 Launch launch_of(bool wide, bool few) {
@@ -620,8 +648,7 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     const int smem = L.smem + (int)a->nb * 12;
     cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    const uint64_t fit = L.blocks * sms;
-    e = qw_launch(L.core, (uint32_t)(most < fit ? most : fit), 128, smem, st, tm, d, k, box_rows, status);
+    e = qw_launch(L.core, (uint32_t)(most < sms ? most : sms), L.threads, smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess || mc < 2) return e;
     return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
 }
