@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
             }
         };
         bool more = lane < X::WARPS && fat < hi;
-        if (lane < X::WARPS) has[lane] = more;
+        if (lane < X::WARPS) has[lane] = more ? fr * c.kvh + fh + 1 : 0;  // the first task's row and kv head
         __syncthreads();
         if (more) ask();
         uint64_t *bars = bars_of(lane < X::WARPS ? lane : 0);
@@ -294,6 +294,48 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
     float fac[NT][2], o[X::CH][NT][4], M[NT][2], l[NT][2];
     const uint32_t Kb = tiles_of(warp), Vb = Kb + RING * X::TILE;
     uint64_t *bars = bars_of(warp);
+    auto load_queries = [&](uint32_t r, uint32_t h) {
+        // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
+        have_r = r, have_h = h;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const uint32_t head = nt * 8 + g;
+            const T *qp = (const T *)a.q + (int64_t)r * a.q_row + (int64_t)(h * a.G + min(head, a.G - 1)) * a.q_head;
+            uint32_t m = 0;
+#pragma unroll
+            for (int cc = 0; cc < HD / 64; cc++) {
+                const int d0 = HD == 64 ? 16 * t : 128 * (cc >> 1) + 16 * (2 * t + (cc & 1));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    uint32_t w[4];
+                    kv8_load_raw8(qp + d0 + 8 * e, w);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        qf[nt][cc * 8 + e * 4 + x] = w[x];
+                        const float2 f = kv8_float2<T>(w[x]);
+                        m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                    }
+                }
+            }
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const uint32_t ex = min(max(m >> 23, 1u), 253u);
+            const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+#pragma unroll
+            for (int x = 0; x < HD / 8; x++) {
+                const float2 f = kv8_float2<T>(qf[nt][x]);
+                const __half2 h2 = __floats2half2_rn(f.x * down, f.y * down);
+                qf[nt][x] = head < a.G ? *(const uint32_t *)&h2 : 0u;
+            }
+            const float f = up * a.scale2;
+            fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+            fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+        }
+    };
+    {
+        const uint32_t f = has[warp] - 1;  // the first task's, while its tile is on its way
+        load_queries(f / c.kvh, f % c.kvh);
+    }
     for (; more; n++) {
         const uint32_t sl = n % RING;
         if (!mbar_wait(&bars[sl], n / RING & 1)) {
@@ -303,44 +345,7 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         const uint4 in = info_of(warp)[2 * sl], task = info_of(warp)[2 * sl + 1];
         more = !(task.w & 4);
         if (task.w & 1) {
-            if (task.x != have_r || task.y != have_h) {
-                // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
-                have_r = task.x, have_h = task.y;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const uint32_t head = nt * 8 + g;
-                    const T *qp = (const T *)a.q + (int64_t)task.x * a.q_row + (int64_t)(task.y * a.G + min(head, a.G - 1)) * a.q_head;
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int cc = 0; cc < HD / 64; cc++) {
-                        const int d0 = HD == 64 ? 16 * t : 128 * (cc >> 1) + 16 * (2 * t + (cc & 1));
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            uint32_t w[4];
-                            kv8_load_raw8(qp + d0 + 8 * e, w);
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                qf[nt][cc * 8 + e * 4 + x] = w[x];
-                                const float2 f = kv8_float2<T>(w[x]);
-                                m = max(m, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-                            }
-                        }
-                    }
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    const uint32_t ex = min(max(m >> 23, 1u), 253u);
-                    const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
-#pragma unroll
-                    for (int x = 0; x < HD / 8; x++) {
-                        const float2 f = kv8_float2<T>(qf[nt][x]);
-                        const __half2 h2 = __floats2half2_rn(f.x * down, f.y * down);
-                        qf[nt][x] = head < a.G ? *(const uint32_t *)&h2 : 0u;
-                    }
-                    const float f = up * a.scale2;
-                    fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
-                    fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-                }
-            }
+            if (task.x != have_r || task.y != have_h) load_queries(task.x, task.y);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -350,70 +355,85 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
             }
         }
         // ---- scores
-        float s[2][NT][4];
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
-#pragma unroll
-        for (int cc = 0; cc < HD / 64; cc++)
-#pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
-                const uint32_t ad = Kb + sl * X::TILE + (HD == 64 ? (mt * 16 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4) : (cc >> 1) * STEP * 128 + (mt * 16 + g) * 128 + (((2 * t + (cc & 1)) ^ g) << 4));
-                uint32_t v[4], u[4];
-                lds128(v, ad);
-                lds128(u, ad + 8 * X::BOX);
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    uint32_t af[4];
-                    kv8_operands<FMT>(v[x], af[0], af[2]);
-                    kv8_operands<FMT>(u[x], af[1], af[3]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma_f16(s[mt][nt], af, qf[nt][cc * 8 + 2 * x], qf[nt][cc * 8 + 2 * x + 1], s[mt][nt]);
-                }
-            }
-        float ks[2][2], lv[2][2], x1[NT][2];
+        const uint32_t cnt[2] = {in.x >> 16 ? 0u : in.x, in.y >> 16 ? 0u : in.y};  // valid tokens of either 16
+        float kf[2][NT][4], lv[2][2];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const float *sc = scales_of(warp) + sl * 2 * STEP + mt * 16 + g + 8 * e;
-                ks[mt][e] = sc[0], lv[mt][e] = sc[STEP];
-            }
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) x1[nt][0] = x1[nt][1] = -INFINITY;
-        const uint32_t cnt[2] = {in.x >> 16 ? 0u : in.x, in.y >> 16 ? 0u : in.y};  // valid tokens of either 16
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++) {
-            const bool bad = (mt ? in.y : in.x) >> 16;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const bool have = g + 8 * e < cnt[mt];
-                const float vscale = lv[mt][e];
-                const bool nan = bad || (have && vscale != vscale);  // (a key's scale that is no number makes the score one by itself)
+                const float kscale = sc[0], vscale = sc[STEP];
                 // a scale below 2^-110, which put does not make, counts as 2^-110 here
-                lv[mt][e] = !have ? -INFINITY : vscale < LOWEST ? LOWEST_LOG2 : __log2f(vscale);
+                lv[mt][e] = vscale < LOWEST ? LOWEST_LOG2 : __log2f(vscale);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int d = 0; d < 2; d++) {
-                        float &v = s[mt][nt][2 * e + d];
-                        v = nan ? __uint_as_float(0x7fffffffu) : have ? v * (ks[mt][e] * fac[nt][d]) : -INFINITY;
-                        if (have) x1[nt][d] = fmaxf(x1[nt][d], v + lv[mt][e]);
+                    for (int d = 0; d < 2; d++) kf[mt][nt][2 * e + d] = kscale * fac[nt][d];
+            }
+        float s[2][NT][4];
+        {
+            constexpr int CHAINS = HD == 64 ? 1 : 2;  // a product waits for the one before it in its sum
+            float sa[CHAINS][2][NT][4];
+#pragma unroll
+            for (int y = 0; y < CHAINS; y++)
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) sa[y][mt][nt][0] = sa[y][mt][nt][1] = sa[y][mt][nt][2] = sa[y][mt][nt][3] = 0.f;
+#pragma unroll
+            for (int cc = 0; cc < HD / 64; cc++) {
+                uint32_t v[2][4], u[2][4];
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++) {
+                    const uint32_t ad = Kb + sl * X::TILE + (HD == 64 ? (mt * 16 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4) : (cc >> 1) * STEP * 128 + (mt * 16 + g) * 128 + (((2 * t + (cc & 1)) ^ g) << 4));
+                    lds128(v[mt], ad);
+                    lds128(u[mt], ad + 8 * X::BOX);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int mt = 0; mt < 2; mt++) {
+                        uint32_t af[4];
+                        kv8_operands<FMT>(v[mt][x], af[0], af[2]);
+                        kv8_operands<FMT>(u[mt][x], af[1], af[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            float(&y)[4] = sa[x % CHAINS][mt][nt];
+                            mma_f16(y, af, qf[nt][cc * 8 + 2 * x], qf[nt][cc * 8 + 2 * x + 1], y);
+                        }
                     }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[2 * RING + sl]);
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[mt][nt][x] = (sa[0][mt][nt][x] + (CHAINS > 1 ? sa[CHAINS - 1][mt][nt][x] : 0.f)) * kf[mt][nt][x];
         }
+        if (cnt[0] + cnt[1] < 32) {  // rows behind the last token, and tokens that are not in the cache
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (g + 8 * e >= cnt[mt]) {
+                        lv[mt][e] = -INFINITY;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) s[mt][nt][2 * e] = s[mt][nt][2 * e + 1] = (mt ? in.y : in.x) >> 16 ? __uint_as_float(0x7fffffffu) : -INFINITY;
+                    }
+        }
+        float x1[NT][2];
         bool up = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
+                x1[nt][d] = fmaxf(fmaxf(s[0][nt][d] + lv[0][0], s[0][nt][2 + d] + lv[0][1]), fmaxf(s[1][nt][d] + lv[1][0], s[1][nt][2 + d] + lv[1][1]));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x1[nt][d] = fmaxf(x1[nt][d], __shfl_xor_sync(0xffffffffu, x1[nt][d], off));
                 up |= x1[nt][d] > M[nt][d];
             }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[2 * RING + sl]);
         if (__any_sync(0xffffffffu, up)) {  // a larger maximum
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -437,10 +457,10 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                 for (int e = 0; e < 2; e++)
 #pragma unroll
                     for (int d = 0; d < 2; d++) {
-                        const float v = s[mt][nt][2 * e + d], off = v - M[nt][d];
-                        const bool none = v == -INFINITY;
-                        l[nt][d] += none ? 0.f : exp2_fast(off);
-                        wt[2 * e + d] = none ? 0.f : exp2_fast(off + lv[mt][e]);
+                        // (nothing so far: M is -infinity, and so is every score, or a NaN)
+                        const float off = s[mt][nt][2 * e + d] - (M[nt][d] == -INFINITY ? 0.f : M[nt][d]);
+                        l[nt][d] += exp2_fast(off);
+                        wt[2 * e + d] = exp2_fast(off + lv[mt][e]);
                     }
                 const __half2 h01 = __floats2half2_rn(wt[0], wt[1]), h23 = __floats2half2_rn(wt[2], wt[3]);
                 const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
@@ -525,17 +545,69 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// A block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  Bound: the latency of
-// two rounds of loads -- a first form with a block per head went through 188 chunks (48000 tokens) in 47 dependent rounds.  grid (qh hd / 64, nb) x 256
+// Up to 32 chunks: a warp per (head, row), a lane knows one chunk's weight.  The operations of a row are those of kv8_merge_k in the same order.  grid ceil(nb qh / 8) x 256
+template <int HD, class T>
+__global__ void __launch_bounds__(256) kv8_merge_few_k(Kv8Dev c, AttnArgs a) {
+    constexpr int E = HD / 128 ? HD / 128 : 1;  // 16-byte pieces of a lane
+    pdl_sync();
+    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = x / a.qh, qh = x % a.qh;
+    if (r >= a.nb) return;
+    const int len = a.lens[r];
+    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], len));
+    if (nch < 2) return;  // written by the core
+    const float2 st = lane < nch ? __ldcg(stats_of(a, HD, r, qh) + lane) : make_float2(-INFINITY, 0.f);
+    const float *p = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + 4 * lane;
+    const size_t cs = (size_t)a.qh * HD;
+    float4 acc[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float M = warp_max(st.x), w = st.x == -INFINITY ? 0.f : exp2f(st.x - M);
+    const float l = warp_sum(st.x == -INFINITY ? st.y : st.y * w);  // (0, or NaN, where a chunk has no maximum)
+    const bool mine = HD >= 128 || lane < HD / 4;
+#pragma unroll 8
+    for (uint32_t k = 0; k < 16; k++) {
+        if (k >= nch) break;  // (the same in all lanes)
+        const float w0 = __shfl_sync(0xffffffffu, w, k), w1 = __shfl_sync(0xffffffffu, w, k + 16);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 v = mine ? __ldcg((const float4 *)(p + k * cs + 128 * i)) : z, u = mine && k + 16 < nch ? __ldcg((const float4 *)(p + (k + 16) * cs + 128 * i)) : z;
+            acc[i].x += fmaf(u.x, w1, v.x * w0), acc[i].y += fmaf(u.y, w1, v.y * w0), acc[i].z += fmaf(u.z, w1, v.z * w0), acc[i].w += fmaf(u.w, w1, v.w * w0);
+        }
+    }
+    const bool bad = (uint32_t)len > a.max_len;
+    if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
+    if (!mine) return;
+#pragma unroll
+    for (int i = 0; i < E; i++) finish<T>(a, r, qh, 128 * i + 4 * lane, acc[i], bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
+}
+
+// More: a block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  The first eight loads
+// of a thread leave before the weights are known.  (A first form with a block per head went through 188 chunks, 48000 tokens, in 47 dependent rounds: 30 us.)
+// grid (qh hd / 64, nb) x 256
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     __shared__ float4 accs[16][16];
     __shared__ float wm[8], wl[8];
     pdl_sync();
     const uint32_t qh = blockIdx.x / (HD / 64), ch = blockIdx.x % (HD / 64) * 64, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % 16, cg = tid / 16;
-    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], a.lens[r]));
+    const int len = a.lens[r];
+    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], len));
     if (nch < 2) return;  // written by the core
     const float2 *st = stats_of(a, HD, r, qh);
+    const float4 *p = (const float4 *)(a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch) + wc;
+    const size_t cs = (size_t)a.qh * (HD / 4);
+    float4 v[8];
+    float Mv[8];
+    auto load = [&](uint32_t k0) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t k = k0 + 16 * i;
+            Mv[i] = k < nch ? __ldcg(&st[k].x) : -INFINITY;
+            v[i] = k < nch ? __ldcg(p + k * cs) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    load(cg);
     float M = -INFINITY;
     for (uint32_t k = tid; k < nch; k += 256) M = fmaxf(M, __ldcg(&st[k].x));
     M = warp_max(M);
@@ -550,14 +622,15 @@ __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     }
     l = warp_sum(l);
     if (lane == 0) wl[warp] = l;
-    const float4 *p = (const float4 *)(a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch) + wc;
-    const size_t cs = (size_t)a.qh * (HD / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (uint32_t k = cg; k < nch; k += 16) {
-        const float Mk = __ldcg(&st[k].x), w = Mk == -INFINITY ? 0.f : exp2f(Mk - M);
-        const float4 v = __ldcg(p + k * cs);
-        acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
+    for (uint32_t k0 = cg; k0 < nch;) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float w = Mv[i] == -INFINITY ? 0.f : exp2f(Mv[i] - M);
+            acc.x = fmaf(v[i].x, w, acc.x), acc.y = fmaf(v[i].y, w, acc.y), acc.z = fmaf(v[i].z, w, acc.z), acc.w = fmaf(v[i].w, w, acc.w);
+        }
+        k0 += 128;
+        if (k0 < nch) load(k0);
     }
     accs[cg][wc] = acc;
     __syncthreads();
@@ -567,10 +640,10 @@ __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     for (int w = 1; w < 8; w++) l += wl[w];
 #pragma unroll
     for (int g = 1; g < 16; g++) {
-        const float4 v = accs[g][tid];
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        const float4 u = accs[g][tid];
+        acc.x += u.x, acc.y += u.y, acc.z += u.z, acc.w += u.w;
     }
-    const bool bad = (uint32_t)a.lens[r] > a.max_len;
+    const bool bad = (uint32_t)len > a.max_len;
     if (bad && tid == 0) set_status(c.status, ST_BAD_ARG | 0x24);
     finish<T>(a, r, qh, ch + 4 * tid, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
 }
@@ -580,12 +653,12 @@ typedef void (*core_kernel)(CUtensorMap, Kv8Dev, AttnArgs, uint32_t, unsigned *)
 typedef void (*merge_kernel)(Kv8Dev, AttnArgs);
 struct Launch {
     core_kernel core;
-    merge_kernel merge;
+    merge_kernel merge, merge_few;
     int smem, threads;  // shared memory but for 12 bytes per row
 };
 template <int HD, int FMT, class T, int NT, bool FEW>
 Launch launch_of() {
-    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::THREADS};
+    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, kv8_merge_few_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::THREADS};
 }
 template <int HD, int FMT, class T>
 Launch launch_of(bool wide, bool few) {
@@ -650,6 +723,8 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     if (e != cudaSuccess) return e;
     e = qw_launch(L.core, (uint32_t)(most < sms ? most : sms), L.threads, smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess || mc < 2) return e;
+    // 4096 (head, row) pairs of 32 chunks took 16 us in blocks of 64 channels
+    if (mc <= 32) return qw_launch(L.merge_few, (uint32_t)(((uint64_t)a->nb * a->qh + 7) / 8), 256, 0, st, d, k);
     return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
 }
 
