@@ -13,8 +13,9 @@ using namespace qw;
 namespace {
 // Tokens of a chunk, by the tokens of its row alone (a row's result does not depend on the others of a call): short rows in small pieces, for their latency;
 // a chunk of 256 leaves 6 % of its own bytes as fp32 sums.
-__host__ __device__ inline uint32_t chunk_of(uint32_t n) { return n <= 512 ? 32 : n <= 2048 ? 64 : n <= 8192 ? 128 : 256; }
-__host__ __device__ inline uint32_t chunks_in(uint32_t n) { return (n + chunk_of(n) - 1) / chunk_of(n); }
+__host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 8192 ? 7 : 8; }
+__host__ __device__ inline uint32_t chunk_of(uint32_t n) { return 1u << chunk_log(n); }
+__host__ __device__ inline uint32_t chunks_in(uint32_t n) { return (n + chunk_of(n) - 1) >> chunk_log(n); }
 constexpr float LOWEST = 7.7037197775489434e-34f, LOWEST_LOG2 = -110.f;  // 2^-110
 
 struct AttnArgs {
@@ -32,6 +33,15 @@ __device__ __forceinline__ uint32_t row_tokens(const Kv8Dev &c, const AttnArgs &
     if (slot < 0 || len <= 0) return 0;
     const uint32_t n = min((uint32_t)len, a.max_len);
     return a.blocks ? min(a.nblocks, (n + c.block - 1) / c.block) * c.block : n;
+}
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {  // inclusive sums
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= (uint32_t)o) v += u;
+    }
+    return v;
 }
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x: 0 below 2^-126
     float y;
@@ -101,29 +111,29 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
     auto bars_of = [&](uint32_t w) { return (uint64_t *)(smem + X::BARS) + w * RING * 4; };
     for (uint32_t i = tid; i < X::SLOTS * 4; i += X::THREADS) mbar_init((uint64_t *)(smem + X::BARS) + i, 1);
     mbar_init_fence();
+    __syncthreads();
     pdl_sync();
     // ---- rows: steps of one kv head, running sum; length (top bit: longer than the call allows), slot
-    {
+    auto put_row = [&](uint32_t r) {  // returns its steps
+        if (r >= a.nb) return 0u;
+        const int len = a.lens[r], slot = a.slots[r];
+        lenv[r] = len <= 0 ? 0u : (uint32_t)len > a.max_len ? a.max_len | 0x80000000u : (uint32_t)len;
+        slotv[r] = (uint32_t)slot;
+        return (row_tokens(c, a, slot, len) + STEP - 1) / STEP;
+    };
+    if (a.nb <= 64) {  // every warp for itself, all the same values: no barrier (the block's one took 1500 cycles of the 5 us that a row of 100 tokens takes)
+        const uint32_t n0 = put_row(2 * lane), n1 = put_row(2 * lane + 1);
+        const uint32_t at = warp_scan(n0 + n1) - n0 - n1;
+        if (2 * lane <= a.nb) first[2 * lane] = at;
+        if (2 * lane + 1 <= a.nb) first[2 * lane + 1] = at + n0;
+        if (lane == 31 && a.nb == 64) first[64] = at + n0 + n1;
+        __syncwarp();
+    } else {
         constexpr uint32_t PER = (KV8_MAX_ROWS + X::THREADS - 1) / X::THREADS;
         uint32_t n[PER], sum = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const uint32_t r = tid * PER + i;
-            n[i] = 0;
-            if (r < a.nb) {
-                const int len = a.lens[r], slot = a.slots[r];
-                n[i] = (row_tokens(c, a, slot, len) + STEP - 1) / STEP;
-                lenv[r] = len <= 0 ? 0u : (uint32_t)len > a.max_len ? a.max_len | 0x80000000u : (uint32_t)len;
-                slotv[r] = (uint32_t)slot;
-            }
-            sum += n[i];
-        }
-        uint32_t at = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, at, o);
-            if (lane >= (uint32_t)o) at += u;
-        }
+        for (int i = 0; i < PER; i++) sum += n[i] = put_row(tid * PER + i);
+        uint32_t at = warp_scan(sum);
         if (lane == 31) has[warp] = at;
         __syncthreads();
         at -= sum;
@@ -136,34 +146,35 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         }
         __syncthreads();
     }
-    for (uint32_t r = blockIdx.x; r < a.nb; r += gridDim.x)  // rows of length 0
-        if (first[r] == first[r + 1] && (int)slotv[r] >= 0)
-            for (uint32_t i = tid; i < a.qh * HD; i += X::THREADS) ((T *)a.y)[(int64_t)r * a.y_row + (int64_t)(i / HD) * a.y_head + i % HD] = kv8_round<T>(0.f);
 
-    // ---- the feeding warp: lane w has the task whose tiles warp w gets next
-    if (warp == X::WARPS) {
-        const uint32_t total = first[a.nb] * c.kvh, W = gridDim.x * X::WARPS, w0 = lane * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
-        const uint32_t lo = lane < X::WARPS ? (uint32_t)((uint64_t)w0 * total / W) : total, hi = lane < X::WARPS ? (uint32_t)((uint64_t)(w0 + 1) * total / W) : total;
-        uint32_t fr = 0, fh = 0, fch = 0, fat = total;      // row, kv head, chunk; the task's first step
-        uint32_t fsteps = 0, fcs = 1, flen = 0, fn = 0;     // of the row: steps, steps of a chunk, length, tokens (of entries)
-        int fslot = 0;
-        auto row_of = [&]() {
-            fsteps = first[fr + 1] - first[fr];
-            flen = lenv[fr] & 0x7fffffffu;
-            fslot = (int)slotv[fr];
-            fn = row_tokens(c, a, fslot, (int)flen);
-            fcs = chunk_of(fn) / STEP;
-        };
-        auto settle = [&]() {  // after fch or fh may have run over
-            if (fch * fcs >= fsteps) fch = 0, fh++;
-            if (fh >= c.kvh) {
-                fh = 0;
-                do fr++;
-                while (fr < a.nb && first[fr + 1] == first[fr]);
-                if (fr < a.nb) row_of();
-            }
-            fat = fr < a.nb ? first[fr] * c.kvh + fh * fsteps + fch * fcs : total;
-        };
+    // ---- a warp's share, and its first task
+    struct Cursor {
+        uint32_t r, h, ch, at;          // row, kv head, chunk; the task's first step
+        uint32_t steps, cs, len, n;     // of the row: steps, steps of a chunk, length, tokens (of entries)
+        int slot;
+    } f;
+    const uint32_t total = first[a.nb] * c.kvh;
+    auto row_of = [&]() {
+        f.steps = first[f.r + 1] - first[f.r];
+        f.len = lenv[f.r] & 0x7fffffffu;
+        f.slot = (int)slotv[f.r];
+        f.n = row_tokens(c, a, f.slot, (int)f.len);
+        f.cs = chunk_of(f.n) / STEP;
+    };
+    auto settle = [&]() {  // after f.ch or f.h may have run over
+        if (f.ch * f.cs >= f.steps) f.ch = 0, f.h++;
+        if (f.h >= c.kvh) {
+            f.h = 0;
+            do f.r++;
+            while (f.r < a.nb && first[f.r + 1] == first[f.r]);
+            if (f.r < a.nb) row_of();
+        }
+        f.at = f.r < a.nb ? first[f.r] * c.kvh + f.h * f.steps + f.ch * f.cs : total;
+    };
+    auto find = [&](uint32_t w) {  // warp w's; returns the end of its share
+        const uint32_t W = gridDim.x * X::WARPS, w0 = w * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
+        const uint32_t lo = (uint32_t)((uint64_t)w0 * total / W), hi = (uint32_t)((uint64_t)(w0 + 1) * total / W);
+        f.at = total;
         if (lo < hi) {
             uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
             while (u - l > 1) {
@@ -171,33 +182,40 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                 if (first[m] * c.kvh <= lo) l = m;
                 else u = m;
             }
-            fr = l;
+            f.r = l;
             row_of();
-            const uint32_t rem = lo - first[fr] * c.kvh;
-            fh = rem / fsteps;
-            fch = (rem - fh * fsteps + fcs - 1) / fcs;
+            const uint32_t rem = lo - first[f.r] * c.kvh;
+            f.h = rem / f.steps;
+            f.ch = (rem - f.h * f.steps + f.cs - 1) / f.cs;
             settle();
         }
+        return hi;
+    };
+
+    // ---- the feeding warp: lane w has the task whose tiles warp w gets next
+    if (warp == X::WARPS) {
+        const uint32_t hi = lane < X::WARPS ? find(lane) : 0;
+        bool more = lane < X::WARPS && f.at < hi;
         // a tile: 16 tokens each -- valid ones | 0x10000 (not in the cache), token and page of the first
         uint32_t in[2], tok[2], fstep = 0;
         int page[2];
         auto ask = [&]() {
-            const uint32_t o = (fch * fcs + fstep) * STEP;
+            const uint32_t o = (f.ch * f.cs + fstep) * STEP;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 in[e] = 0;
                 page[e] = -1;
                 uint32_t x = o + 16 * e;
-                if (x >= fn) continue;
+                if (x >= f.n) continue;
                 if (a.blocks) {
                     if (e && box_rows != 16) {  // the same block
                         x = tok[0] + 16;
                         if (!in[0] || in[0] >> 16) continue;
                     } else {
                         const uint32_t en = x / c.block;
-                        const int b = en < a.nblocks ? __ldcg(a.blocks + ((size_t)fr * c.kvh + fh) * a.nblocks + en) : -1;
+                        const int b = en < a.nblocks ? __ldcg(a.blocks + ((size_t)f.r * c.kvh + f.h) * a.nblocks + en) : -1;
                         if (b < 0) continue;
-                        if ((uint32_t)b >= (flen + c.block - 1) / c.block) {
+                        if ((uint32_t)b >= (f.len + c.block - 1) / c.block) {
                             in[e] = 16 | 0x10000u;
                             continue;
                         }
@@ -205,14 +223,11 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                     }
                 }
                 tok[e] = x;
-                if (x >= flen) continue;
-                in[e] = min(16u, flen - x);
-                if ((e == 0 || box_rows == 16) && kv8_entry_ok(c, fslot, x / KV8_PAGE)) page[e] = __ldcg(c.ptab + (size_t)fslot * c.max_pages + x / KV8_PAGE);
+                if (x >= f.len) continue;
+                in[e] = min(16u, f.len - x);
+                if ((e == 0 || box_rows == 16) && kv8_entry_ok(c, f.slot, x / KV8_PAGE)) page[e] = __ldcg(c.ptab + (size_t)f.slot * c.max_pages + x / KV8_PAGE);
             }
         };
-        bool more = lane < X::WARPS && fat < hi;
-        if (lane < X::WARPS) has[lane] = more ? fr * c.kvh + fh + 1 : 0;  // the first task's row and kv head
-        __syncthreads();
         if (more) ask();
         uint64_t *bars = bars_of(lane < X::WARPS ? lane : 0);
         uint4 *info = info_of(lane < X::WARPS ? lane : 0);
@@ -229,19 +244,19 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 #pragma unroll
                 for (int e = 0; e < 2; e++)
                     if (in[e] && !(in[e] >> 16) && (e == 0 || box_rows == 16)) {
-                        if (kv8_page_ok(c, page[e])) row[e] = kv8_row0(c, (uint32_t)page[e], 0, fh) + tok[e] % KV8_PAGE;
+                        if (kv8_page_ok(c, page[e])) row[e] = kv8_row0(c, (uint32_t)page[e], 0, f.h) + tok[e] % KV8_PAGE;
                         else in[e] |= 0x10000u;
                     }
                 if (box_rows != 16 && in[0] >> 16 && in[1]) in[1] |= 0x10000u;
                 if ((in[0] | in[1]) >> 16) set_status(c.status, ST_BAD_ARG | 0x23);
                 const bool on0 = in[0] && !(in[0] >> 16), on1 = box_rows == 16 && in[1] && !(in[1] >> 16);
-                const uint32_t steps = min(fcs, fsteps - fch * fcs), of = (fstep == 0 ? 1u : 0u) | (fstep + 1 == steps ? 2u : 0u), r = fr, h = fh, ch = fch;
+                const uint32_t steps = min(f.cs, f.steps - f.ch * f.cs), of = (fstep == 0 ? 1u : 0u) | (fstep + 1 == steps ? 2u : 0u), r = f.r, h = f.h, ch = f.ch;
                 info[2 * sl] = make_uint4(in[0], in[1], row[0], row[1]);
                 if (++fstep == steps) {
                     fstep = 0;
-                    fch++;
+                    f.ch++;
                     settle();
-                    more = fat < hi;
+                    more = f.at < hi;
                 }
                 info[2 * sl + 1] = make_uint4(r, h, ch, of | (more ? 0u : 4u));
                 mbar_expect_tx(&bars[sl], (on0 + on1) * box_rows * (HD + 8));
@@ -259,14 +274,14 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                 did = true;
             }
             if (vfed < fed && (vfed < RING || mbar_test(&bars[3 * RING + vl], vfed / RING - 1 & 1))) {
-                const uint4 f = info[2 * vl];
-                const bool on0 = f.x && !(f.x >> 16), on1 = box_rows == 16 && f.y && !(f.y >> 16);
+                const uint4 v = info[2 * vl];
+                const bool on0 = v.x && !(v.x >> 16), on1 = box_rows == 16 && v.y && !(v.y >> 16);
                 mbar_expect_tx(&bars[RING + vl], (on0 + on1) * box_rows * HD);
 #pragma unroll
                 for (int e = 0; e < 2; e++)
                     if (e ? on1 : on0) {
 #pragma unroll
-                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? f.w : f.z) + vrows), &bars[RING + vl]);
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? v.w : v.z) + vrows), &bars[RING + vl]);
                     }
                 vfed++;
                 did = true;
@@ -284,8 +299,8 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         }
         return;
     }
-    __syncthreads();
-    if (!has[warp]) return;
+    const uint32_t share_end = find(warp);
+    if (f.at >= share_end) return;
 
     // ---- the computing side
     bool ok = true, more = true;
@@ -332,10 +347,7 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
             fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
         }
     };
-    {
-        const uint32_t f = has[warp] - 1;  // the first task's, while its tile is on its way
-        load_queries(f / c.kvh, f % c.kvh);
-    }
+    load_queries(f.r, f.h);  // the first task's, while its tile is on its way
     for (; more; n++) {
         const uint32_t sl = n % RING;
         if (!mbar_wait(&bars[sl], n / RING & 1)) {
@@ -514,8 +526,9 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[3 * RING + sl]);
         if (task.w & 2) {  // ---- the chunk's totals
-            const uint32_t len = lenv[task.x];
-            const uint32_t nch = chunks_in(row_tokens(c, a, (int)slotv[task.x], (int)(len & 0x7fffffffu)));
+            const size_t at = (size_t)task.x * a.max_chunks + task.z;
+            float *dst = a.part + (at * a.qh + task.y * a.G + 2 * t) * HD + X::LANE * g;
+            float2 *st = stats_of(a, HD, task.x, task.y * a.G + 2 * t) + task.z;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -523,20 +536,14 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                     float lt = l[nt][d];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, off);
-                    const uint32_t head = nt * 8 + 2 * t + d, qh = task.y * a.G + head;
-                    if (head >= a.G) continue;
-                    float *dst = a.part + (((size_t)task.x * a.max_chunks + task.z) * a.qh + qh) * HD;
-                    const float f = len >> 31 ? __uint_as_float(0x7fffffffu) : lt == 0.f ? 0.f : 1.f / lt;
-                    if (nch > 1 && g == 0) stats_of(a, HD, task.x, qh)[task.z] = make_float2(M[nt][d], lt);
+                    if (nt * 8 + 2 * t + d >= a.G) continue;
+                    if (g == 0) st[(nt * 8 + d) * a.max_chunks] = make_float2(M[nt][d], lt);
 #pragma unroll
                     for (int hf = 0; hf < X::HALVES; hf++)
 #pragma unroll
                         for (int x = 0; x < X::LANE / 4; x++) {
                             const float(&y0)[4] = o[hf * 8 + 2 * x][nt], (&y1)[4] = o[hf * 8 + 2 * x + 1][nt];
-                            const float4 v = make_float4(y0[d], y0[2 + d], y1[d], y1[2 + d]);
-                            const uint32_t ch = hf * 128 + X::LANE * g + 4 * x;
-                            if (nch > 1) *(float4 *)(dst + ch) = v;
-                            else finish<T>(a, task.x, qh, ch, v, f);
+                            *(float4 *)(dst + (nt * 8 + d) * HD + hf * 128 + 4 * x) = make_float4(y0[d], y0[2 + d], y1[d], y1[2 + d]);
                         }
                 }
         }
@@ -545,41 +552,41 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Up to 32 chunks: a warp per (head, row), a lane knows one chunk's weight.  The operations of a row are those of kv8_merge_k in the same order.  grid ceil(nb qh / 8) x 256
+// Up to 32 chunks: a warp per 64 channels of a (head, row); 16 lanes take chunks 0 to 15, the others 16 to 31, every load leaves before the weights are known.
+// The operations of a row are those of kv8_merge_k in the same order.  (Rows of length 0 get their zeros here.)  grid ceil(nb qh hd / 512) x 256
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_merge_few_k(Kv8Dev c, AttnArgs a) {
-    constexpr int E = HD / 128 ? HD / 128 : 1;  // 16-byte pieces of a lane
     pdl_sync();
-    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, r = x / a.qh, qh = x % a.qh;
+    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, half = lane >> 4, ch = x % (HD / 64) * 64 + 4 * (lane & 15), y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
     if (r >= a.nb) return;
-    const int len = a.lens[r];
-    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], len));
-    if (nch < 2) return;  // written by the core
+    const int len = a.lens[r], slot = a.slots[r];
+    if (slot < 0) return;
+    const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
     const float2 st = lane < nch ? __ldcg(stats_of(a, HD, r, qh) + lane) : make_float2(-INFINITY, 0.f);
-    const float *p = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + 4 * lane;
+    const float *p = a.part + (((size_t)r * a.max_chunks + 16 * half) * a.qh + qh) * HD + ch;
     const size_t cs = (size_t)a.qh * HD;
-    float4 acc[E];
+    float4 v[16];
 #pragma unroll
-    for (int i = 0; i < E; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t k = 0; k < 16; k++) v[k] = k + 16 * half < nch ? __ldcg((const float4 *)(p + k * cs)) : make_float4(0.f, 0.f, 0.f, 0.f);
     const float M = warp_max(st.x), w = st.x == -INFINITY ? 0.f : exp2f(st.x - M);
     const float l = warp_sum(st.x == -INFINITY ? st.y : st.y * w);  // (0, or NaN, where a chunk has no maximum)
-    const bool mine = HD >= 128 || lane < HD / 4;
-#pragma unroll 8
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
     for (uint32_t k = 0; k < 16; k++) {
-        if (k >= nch) break;  // (the same in all lanes)
-        const float w0 = __shfl_sync(0xffffffffu, w, k), w1 = __shfl_sync(0xffffffffu, w, k + 16);
+        const float wk = __shfl_sync(0xffffffffu, w, k + 16 * half);
+        // chunk k, then chunk k + 16 on top of it, in the upper half's lanes
+        const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        float s[4];
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 v = mine ? __ldcg((const float4 *)(p + k * cs + 128 * i)) : z, u = mine && k + 16 < nch ? __ldcg((const float4 *)(p + (k + 16) * cs + 128 * i)) : z;
-            acc[i].x += fmaf(u.x, w1, v.x * w0), acc[i].y += fmaf(u.y, w1, v.y * w0), acc[i].z += fmaf(u.z, w1, v.z * w0), acc[i].w += fmaf(u.w, w1, v.w * w0);
+        for (int j = 0; j < 4; j++) {
+            const float a0 = __shfl_up_sync(0xffffffffu, e[j] * wk, 16);
+            s[j] = fmaf(e[j], wk, a0);
         }
+        acc.x += s[0], acc.y += s[1], acc.z += s[2], acc.w += s[3];
     }
-    const bool bad = (uint32_t)len > a.max_len;
+    const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
-    if (!mine) return;
-#pragma unroll
-    for (int i = 0; i < E; i++) finish<T>(a, r, qh, 128 * i + 4 * lane, acc[i], bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
+    if (half) finish<T>(a, r, qh, ch, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
 }
 
 // More: a block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  The first eight loads
@@ -591,9 +598,9 @@ __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     __shared__ float wm[8], wl[8];
     pdl_sync();
     const uint32_t qh = blockIdx.x / (HD / 64), ch = blockIdx.x % (HD / 64) * 64, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % 16, cg = tid / 16;
-    const int len = a.lens[r];
-    const uint32_t nch = chunks_in(row_tokens(c, a, a.slots[r], len));
-    if (nch < 2) return;  // written by the core
+    const int len = a.lens[r], slot = a.slots[r];
+    if (slot < 0) return;
+    const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
     const float2 *st = stats_of(a, HD, r, qh);
     const float4 *p = (const float4 *)(a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch) + wc;
     const size_t cs = (size_t)a.qh * (HD / 4);
@@ -643,7 +650,7 @@ __global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
         const float4 u = accs[g][tid];
         acc.x += u.x, acc.y += u.y, acc.z += u.z, acc.w += u.w;
     }
-    const bool bad = (uint32_t)len > a.max_len;
+    const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && tid == 0) set_status(c.status, ST_BAD_ARG | 0x24);
     finish<T>(a, r, qh, ch + 4 * tid, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
 }
@@ -722,9 +729,9 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     e = qw_launch(L.core, (uint32_t)(most < sms ? most : sms), L.threads, smem, st, tm, d, k, box_rows, status);
-    if (e != cudaSuccess || mc < 2) return e;
+    if (e != cudaSuccess) return e;
     // 4096 (head, row) pairs of 32 chunks took 16 us in blocks of 64 channels
-    if (mc <= 32) return qw_launch(L.merge_few, (uint32_t)(((uint64_t)a->nb * a->qh + 7) / 8), 256, 0, st, d, k);
+    if (mc <= 32) return qw_launch(L.merge_few, (uint32_t)(((uint64_t)a->nb * a->qh * (c->hd / 64) + 7) / 8), 256, 0, st, d, k);
     return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
 }
 

@@ -19,6 +19,12 @@ class Kv8Error(RuntimeError):
     pass
 
 
+def _raw_stream(index):
+    """The cudaStream_t of torch's current stream (torch.cuda.current_stream() builds an object around it, 3 us)."""
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 class CacheStruct(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "bounds", "page_table", "status")] + \
                [(n, C.c_uint32) for n in ("pages", "layers", "kvh", "hd", "format", "block", "slots", "max_pages")]
@@ -86,6 +92,7 @@ class Kv8Cache:
             raise Kv8Error("status is one 32-bit word")
         self.tensors = (codes, scales, bounds, page_table, status)
         self.device = codes.device
+        self.index = codes.get_device()
         for t in self.tensors:
             if t is not None and (t.device != self.device or not t.is_contiguous()):
                 raise Kv8Error("a cache's tensors are contiguous and on one device")
@@ -93,45 +100,46 @@ class Kv8Cache:
         self.c = CacheStruct(*ptr, pages, layers, kvh, hd, FORMATS[format], block or 64, page_table.shape[0], page_table.shape[1])
         self.kvh, self.hd, self.slots, self.max_pages = kvh, hd, page_table.shape[0], page_table.shape[1]
         self._err = C.create_string_buffer(256)
+        self._ref = C.byref(self.c)
         if self.L.qw_kv8_bytes(C.byref(self.c), (C.c_size_t * 3)()):
             raise Kv8Error("a cache of these sizes is not supported (head dim 64, 128 or 256; blocks of 16 to 256 tokens)")
 
     # ---- arguments
     def _index(self, t, nb, what):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != nb or not t.is_contiguous() or t.device != self.device:
+        if t.dtype is not torch.int32 or t.shape != (nb,) or not t.is_contiguous() or t.get_device() != self.index:
             raise Kv8Error("%s is int32 [%d] on the cache's device" % (what, nb))
         return t.data_ptr()
 
     def _rows(self, t, nb, heads, dtype, what):
-        if t.dim() != 3 or t.shape[0] != nb or t.shape[1] != heads or t.shape[2] != self.hd or t.dtype != dtype or t.device != self.device:
+        if t.shape != (nb, heads, self.hd) or t.dtype is not dtype or t.get_device() != self.index:
             raise Kv8Error("%s is %s [%d, %d, %d] on the cache's device" % (what, dtype, nb, heads, self.hd))
-        s = t.stride()
-        if s[2] != 1 and self.hd > 1:
+        row, head, one = t.stride()
+        if one != 1:
             raise Kv8Error("the last dimension of %s is contiguous" % what)
-        return t.data_ptr(), s[0], s[1]
+        return t.data_ptr(), row, head
 
     def _blocks(self, t, nb):
-        if t.dtype != torch.int32 or t.dim() != 3 or t.shape[0] != nb or t.shape[1] != self.kvh or not t.is_contiguous() or t.device != self.device:
+        if t.dtype is not torch.int32 or t.dim() != 3 or t.shape[0] != nb or t.shape[1] != self.kvh or not t.is_contiguous() or t.get_device() != self.index:
             raise Kv8Error("blocks are int32 [%d, %d, n] on the cache's device" % (nb, self.kvh))
         return t.data_ptr(), t.shape[2]
 
     def _work(self, work, need):
         if work is None:
             work = torch.empty(max(16, need), dtype=torch.uint8, device=self.device)
-        if work.device != self.device or not work.is_contiguous():
+        if work.get_device() != self.index or not work.is_contiguous():
             raise Kv8Error("the workspace is contiguous and on the cache's device")
         return work, work.data_ptr(), work.numel() * work.element_size()
 
     def _call(self, fn, args, stream):
-        if self.device.type != "cuda":
+        if self.index < 0:
             raise Kv8Error("the cache is not in device memory (this library has no CPU path)")
         if stream is None:
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(C.byref(self.c), C.byref(args), stream, self._err, 256)
+            stream = _raw_stream(self.index)
+        if torch.cuda.current_device() == self.index:
+            rc = fn(self._ref, C.byref(args), stream, self._err, 256)
         else:
             with torch.cuda.device(self.device):
-                rc = fn(C.byref(self.c), C.byref(args), stream, self._err, 256)
+                rc = fn(self._ref, C.byref(args), stream, self._err, 256)
         if rc:
             raise Kv8Error(self._err.value.decode())
 
@@ -150,49 +158,38 @@ class Kv8Cache:
             raise Kv8Error("sizes that the calls refuse")
         return max(n, self.L.qw_kv8_pick_work(C.byref(self.c), nb, max_len))
 
+    def _rows_call(self, fn, k, v, slots, pos, layer, stream):
+        nb, dt = slots.shape[0], self._dtype(k, "k")
+        kp, kr, kh = self._rows(k, nb, self.kvh, k.dtype, "k")
+        vp, vr, vh = self._rows(v, nb, self.kvh, k.dtype, "v")
+        self._call(fn, RowsStruct(kp, vp, self._index(slots, nb, "slots"), self._index(pos, nb, "pos"), kr, kh, vr, vh, nb, layer, dt), stream)
+
     def put(self, k, v, slots, pos, layer=0, stream=None):
         """Quantises rows k, v [nb, kvh, hd] into position pos[r] of slot slots[r], and renews the bounds of their blocks."""
-        nb, dt = slots.shape[0], self._dtype(k, "k")
-        a = RowsStruct()
-        a.k, a.k_row, a.k_head = self._rows(k, nb, self.kvh, k.dtype, "k")
-        a.v, a.v_row, a.v_head = self._rows(v, nb, self.kvh, k.dtype, "v")
-        a.slots, a.pos, a.nb, a.layer, a.dtype = self._index(slots, nb, "slots"), self._index(pos, nb, "pos"), nb, layer, dt
-        self._call(self.L.qw_kv8_put, a, stream)
+        self._rows_call(self.L.qw_kv8_put, k, v, slots, pos, layer, stream)
 
     def get(self, k, v, slots, pos, layer=0, stream=None):
         """Reads rows back into k, v [nb, kvh, hd]."""
-        nb, dt = slots.shape[0], self._dtype(k, "k")
-        a = RowsStruct()
-        a.k, a.k_row, a.k_head = self._rows(k, nb, self.kvh, k.dtype, "k")
-        a.v, a.v_row, a.v_head = self._rows(v, nb, self.kvh, k.dtype, "v")
-        a.slots, a.pos, a.nb, a.layer, a.dtype = self._index(slots, nb, "slots"), self._index(pos, nb, "pos"), nb, layer, dt
-        self._call(self.L.qw_kv8_get, a, stream)
+        self._rows_call(self.L.qw_kv8_get, k, v, slots, pos, layer, stream)
 
     def attn(self, q, lens, slots, y, layer=0, *, max_len, scale=None, gate=None, blocks=None, work=None, stream=None):
         """y [nb, qh, hd] = attention of q over the first lens[r] tokens of slot slots[r] (of the blocks [nb, kvh, n], if given), times sigmoid(gate)."""
         nb, qh, dt = lens.shape[0], q.shape[1] if q.dim() == 3 else 0, self._dtype(q, "q")
-        a = AttnStruct()
-        a.q, a.q_row, a.q_head = self._rows(q, nb, qh, q.dtype, "q")
-        a.y, a.y_row, a.y_head = self._rows(y, nb, qh, q.dtype, "y")
-        if gate is not None:
-            a.gate, a.gate_row, a.gate_head = self._rows(gate, nb, qh, q.dtype, "gate")
-        a.lens, a.slots = self._index(lens, nb, "lens"), self._index(slots, nb, "slots")
-        if blocks is not None:
-            a.blocks, a.nblocks = self._blocks(blocks, nb)
-        work, a.work, a.work_bytes = self._work(work, self.L.qw_kv8_attn_work(C.byref(self.c), nb, qh, max_len, a.nblocks) if work is None else 0)
-        a.scale = self.hd ** -0.5 if scale is None else scale
-        a.nb, a.layer, a.dtype, a.qh, a.max_len = nb, layer, dt, qh, max_len
-        self._call(self.L.qw_kv8_attn, a, stream)
+        qp, qr, qd = self._rows(q, nb, qh, q.dtype, "q")
+        yp, yr, yd = self._rows(y, nb, qh, q.dtype, "y")
+        gp, gr, gd = (None, 0, 0) if gate is None else self._rows(gate, nb, qh, q.dtype, "gate")
+        bp, nblocks = (None, 0) if blocks is None else self._blocks(blocks, nb)
+        work, wp, size = self._work(work, self.L.qw_kv8_attn_work(self._ref, nb, qh, max_len, nblocks) if work is None else 0)
+        self._call(self.L.qw_kv8_attn, AttnStruct(qp, gp, yp, self._index(lens, nb, "lens"), self._index(slots, nb, "slots"), bp, wp, size, qr, qd, gr, gd, yr, yd,
+                                                  self.hd ** -0.5 if scale is None else scale, nb, layer, dt, qh, max_len, nblocks), stream)
         return y
 
     def pick(self, q, lens, slots, blocks, layer=0, *, max_len, first=0, last=1, work=None, stream=None):
         """blocks [nb, kvh, n]: the block numbers with the best scores for q, ascending, the first `first` and the last `last` always among them."""
         nb, qh, dt = lens.shape[0], q.shape[1] if q.dim() == 3 else 0, self._dtype(q, "q")
-        a = PickStruct()
-        a.q, a.q_row, a.q_head = self._rows(q, nb, qh, q.dtype, "q")
-        a.lens, a.slots = self._index(lens, nb, "lens"), self._index(slots, nb, "slots")
-        a.blocks, a.nblocks = self._blocks(blocks, nb)
-        work, a.work, a.work_bytes = self._work(work, self.L.qw_kv8_pick_work(C.byref(self.c), nb, max_len) if work is None else 0)
-        a.nb, a.layer, a.dtype, a.qh, a.max_len, a.first, a.last = nb, layer, dt, qh, max_len, first, last
-        self._call(self.L.qw_kv8_pick, a, stream)
+        qp, qr, qd = self._rows(q, nb, qh, q.dtype, "q")
+        bp, nblocks = self._blocks(blocks, nb)
+        work, wp, size = self._work(work, self.L.qw_kv8_pick_work(self._ref, nb, max_len) if work is None else 0)
+        self._call(self.L.qw_kv8_pick, PickStruct(qp, self._index(lens, nb, "lens"), self._index(slots, nb, "slots"), bp, wp, size, qr, qd, nb, layer, dt, qh, max_len, nblocks,
+                                                  first, last), stream)
         return blocks
