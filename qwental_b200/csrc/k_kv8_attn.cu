@@ -552,41 +552,40 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Up to 32 chunks: a warp per 64 channels of a (head, row); 16 lanes take chunks 0 to 15, the others 16 to 31, every load leaves before the weights are known.
+// Up to 32 chunks: a warp per 64 channels of a (head, row), two channels and one chunk's weight per lane; every load leaves before the weights are known.
 // The operations of a row are those of kv8_merge_k in the same order.  (Rows of length 0 get their zeros here.)  grid ceil(nb qh hd / 512) x 256
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_merge_few_k(Kv8Dev c, AttnArgs a) {
     pdl_sync();
-    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, half = lane >> 4, ch = x % (HD / 64) * 64 + 4 * (lane & 15), y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
+    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, ch = x % (HD / 64) * 64 + 2 * lane, y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
     if (r >= a.nb) return;
     const int len = a.lens[r], slot = a.slots[r];
     if (slot < 0) return;
     const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
     const float2 st = lane < nch ? __ldcg(stats_of(a, HD, r, qh) + lane) : make_float2(-INFINITY, 0.f);
-    const float *p = a.part + (((size_t)r * a.max_chunks + 16 * half) * a.qh + qh) * HD + ch;
-    const size_t cs = (size_t)a.qh * HD;
-    float4 v[16];
+    const float *p = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch;
+    const uint32_t cs = a.qh * HD;
+    float2 gate = make_float2(0.f, 0.f);
+    const T *gp = (const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch;
+    if (a.gate) gate = make_float2(kv8_float(gp[0]), kv8_float(gp[1]));
+    float2 v[32];
 #pragma unroll
-    for (uint32_t k = 0; k < 16; k++) v[k] = k + 16 * half < nch ? __ldcg((const float4 *)(p + k * cs)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t k = 0; k < 32; k++) v[k] = k < nch ? __ldcg((const float2 *)(p + (size_t)k * cs)) : make_float2(0.f, 0.f);
     const float M = warp_max(st.x), w = st.x == -INFINITY ? 0.f : exp2f(st.x - M);
     const float l = warp_sum(st.x == -INFINITY ? st.y : st.y * w);  // (0, or NaN, where a chunk has no maximum)
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (uint32_t k = 0; k < 16; k++) {
-        const float wk = __shfl_sync(0xffffffffu, w, k + 16 * half);
-        // chunk k, then chunk k + 16 on top of it, in the upper half's lanes
-        const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-        float s[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float a0 = __shfl_up_sync(0xffffffffu, e[j] * wk, 16);
-            s[j] = fmaf(e[j], wk, a0);
-        }
-        acc.x += s[0], acc.y += s[1], acc.z += s[2], acc.w += s[3];
+        const float w0 = __shfl_sync(0xffffffffu, w, k), w1 = __shfl_sync(0xffffffffu, w, k + 16);
+        acc.x += fmaf(v[k + 16].x, w1, __fmul_rn(v[k].x, w0));
+        acc.y += fmaf(v[k + 16].y, w1, __fmul_rn(v[k].y, w0));
     }
     const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
-    if (half) finish<T>(a, r, qh, ch, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
+    const float f = bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l;
+    float out[2] = {acc.x * f, acc.y * f};
+    if (a.gate) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));
+    kv8_store<2>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, out);
 }
 
 // More: a block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  The first eight loads

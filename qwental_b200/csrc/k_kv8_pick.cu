@@ -13,7 +13,7 @@ struct PickArgs {
     int64_t q_row, q_head;
     uint32_t nb, qh, G, max_len, count, first, last, stride;
 };
-constexpr uint32_t RECORDS = 64;  // of a block of threads
+constexpr uint32_t RECORDS = 128;  // of a block of threads
 
 __device__ __forceinline__ uint32_t row_blocks(const Kv8Dev &c, const PickArgs &a, int slot, int len) {
     return slot < 0 || len <= 0 ? 0 : (min((uint32_t)len, a.max_len) + c.block - 1) / c.block;
@@ -24,26 +24,29 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Scores as keys.  A warp has eight consecutive records and asks for all of them before it scores the first; a record is one load of the warp: half of its lanes
-// the lower bounds, which the negative parts of q8 meet, the others the upper ones and the positive parts.  Four products at a time (dp4a), sums of whole
-// numbers across the warp.  Bound: the latency of page id and record, then the bytes of the records (one record after the other took 27 us for 100,000).
-// grid (ceil(most blocks / 64), kvh, nb) x 256
+// Scores as keys: the products of 16 records and 8 heads at a time on the tensor cores (mma m16n8k32 on int8: sums of whole numbers, exact).  A record is
+// [lower | upper bounds], a head's row [negative parts of q8 | positive parts].  Which byte is which k is free as long as both sides agree, so a lane takes 16
+// bytes of a record with one load, all of them before the first product.  Bound: the latency of page id and record, then the bytes of the records.
+// (dp4a with a sum across the warp for every head: 27 us for 100,000 records one after the other, 15 with eight in flight.)
+// grid (ceil(most blocks / 128), kvh, nb) x 256
 template <int HD, class T>
 __global__ void __launch_bounds__(256) kv8_score_k(Kv8Dev c, PickArgs a) {
-    constexpr int E = HD / 16, W = E / 4, PER = RECORDS / 8;  // bytes and words of a record per lane, records of a warp
-    __shared__ __align__(16) int8_t q8[16][2][HD];            // negative parts, positive parts
+    constexpr int CC = 2 * HD / 64, STRIDE = 2 * HD + 64;  // a head's bytes: 64 more, so that neighbouring heads are in other banks
+    __shared__ __align__(16) int8_t q8[16 * STRIDE];
     __shared__ float sqs[16];
     pdl_sync();
-    const uint32_t h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int len = a.lens[r], slot = a.slots[r];
-    const uint32_t n = row_blocks(c, a, slot, len), per = KV8_PAGE / c.block, b0 = blockIdx.x * RECORDS + warp * PER;
+    const uint32_t n = row_blocks(c, a, slot, len), per = KV8_PAGE / c.block, b0 = blockIdx.x * RECORDS + warp * 16;
     if (blockIdx.x * RECORDS >= n) return;
-    // records of the warp, lanes 0 to 7 ask for their pages
-    const uint32_t mine = b0 + (lane & (PER - 1));
-    const int page = mine < n ? kv8_page(c, slot, (int)(mine / per)) : -1;
-    for (uint32_t g = warp; g < a.G; g += 8) {
+    int page[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) page[e] = b0 + g + 8 * e < n ? kv8_page(c, slot, (int)((b0 + g + 8 * e) / per)) : -1;
+    for (uint32_t k = warp; k < 16; k += 8) {  // (heads beyond the last are zeros)
         float x[HD / 32];
-        kv8_load<HD / 32>((const T *)a.q + (int64_t)r * a.q_row + (int64_t)(h * a.G + g) * a.q_head + lane * (HD / 32), x);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) x[i] = 0.f;
+        if (k < a.G) kv8_load<HD / 32>((const T *)a.q + (int64_t)r * a.q_row + (int64_t)(h * a.G + k) * a.q_head + lane * (HD / 32), x);
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
@@ -54,97 +57,84 @@ __global__ void __launch_bounds__(256) kv8_score_k(Kv8Dev c, PickArgs a) {
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             const int v = none ? 0 : __float2int_rn(__fmul_rn(x[i], inv));
-            q8[g][0][lane * (HD / 32) + i] = (int8_t)min(v, 0);
-            q8[g][1][lane * (HD / 32) + i] = (int8_t)max(v, 0);
+            q8[k * STRIDE + lane * (HD / 32) + i] = (int8_t)min(v, 0);
+            q8[k * STRIDE + HD + lane * (HD / 32) + i] = (int8_t)max(v, 0);
         }
-        if (lane == 0) sqs[g] = none ? 0.f : __fdiv_rn(am, 127.f);
+        if (lane == 0) sqs[k] = none ? 0.f : __fdiv_rn(am, 127.f);
     }
-    uint32_t w[PER][W];
-    float sb[PER];
+    uint4 w[2][CC];
+    float sb[2];
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int pg = __shfl_sync(0xffffffffu, page, i);
-        sb[i] = 0.f;
+    for (int e = 0; e < 2; e++) {
+        const uint8_t *rec = c.bounds + kv8_bound_at(c, page[e] < 0 ? 0 : page[e], h, (b0 + g + 8 * e) % per);
+        sb[e] = page[e] < 0 ? 0.f : __ldcg((const float *)(rec + 2 * HD));
 #pragma unroll
-        for (int j = 0; j < W; j++) w[i][j] = 0;
-        if (pg < 0) continue;
-        const uint8_t *rec = c.bounds + kv8_bound_at(c, pg, h, (b0 + i) % per);
-        sb[i] = __ldcg((const float *)(rec + 2 * HD));
-        if (W == 4) {
-            const uint4 v = __ldcg((const uint4 *)rec + lane);
-            w[i][0] = v.x, w[i][W > 1 ? 1 : 0] = v.y, w[i][W > 2 ? 2 : 0] = v.z, w[i][W > 3 ? 3 : 0] = v.w;
-        } else if (W == 2) {
-            const uint2 v = __ldcg((const uint2 *)rec + lane);
-            w[i][0] = v.x, w[i][W > 1 ? 1 : 0] = v.y;
-        } else w[i][0] = __ldcg((const uint32_t *)rec + lane);
+        for (int cc = 0; cc < CC; cc++) w[e][cc] = page[e] < 0 ? make_uint4(0, 0, 0, 0) : __ldcg((const uint4 *)(rec + 64 * cc + 16 * t));
     }
     __syncthreads();
-    float best[PER];
+    float best[2] = {-INFINITY, -INFINITY};
+    for (uint32_t k0 = 0; k0 < a.G; k0 += 8) {
+        int d[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < PER; i++) best[i] = -INFINITY;
-    for (uint32_t g = 0; g < a.G; g++) {
-        int q[W];
+        for (int cc = 0; cc < CC; cc++) {
+            const uint4 q = *(const uint4 *)(q8 + (k0 + g) * STRIDE + 64 * cc + 16 * t);
+            mma_s8(d, w[0][cc].x, w[1][cc].x, w[0][cc].y, w[1][cc].y, q.x, q.y);
+            mma_s8(d, w[0][cc].z, w[1][cc].z, w[0][cc].w, w[1][cc].w, q.z, q.w);
+        }
 #pragma unroll
-        for (int j = 0; j < W; j++) q[j] = *(const int *)(&q8[g][0][0] + lane * E + 4 * j);
-        const float sq = sqs[g];
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            int s = 0;
-#pragma unroll
-            for (int j = 0; j < W; j++) s = __dp4a((int)w[i][j], q[j], s);
-            s = __reduce_add_sync(0xffffffffu, s);
-            best[i] = fmaxf(best[i], s ? __fmul_rn(__fmul_rn(sq, sb[i]), (float)s) : 0.f);
+        for (int j = 0; j < 4; j++) {  // record g + 8 (j / 2), head 2 t + j % 2
+            const uint32_t k = k0 + 2 * t + (j & 1);
+            if (k < a.G) best[j >> 1] = fmaxf(best[j >> 1], d[j] ? __fmul_rn(__fmul_rn(sqs[k], sb[j >> 1]), (float)d[j]) : 0.f);
         }
     }
-    uint32_t key = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (lane == (uint32_t)i) key = key_of(sb[i] == INFINITY ? INFINITY : best[i]);
-    if (lane < PER && mine < n) {
-        if (page < 0) {
+    for (int e = 0; e < 2; e++) {
+        best[e] = fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 1));
+        best[e] = fmaxf(best[e], __shfl_xor_sync(0xffffffffu, best[e], 2));
+        const uint32_t b = b0 + g + 8 * e;
+        if (t || b >= n) continue;
+        uint32_t key = key_of(sb[e] == INFINITY ? INFINITY : best[e]);
+        if (page[e] < 0) {
             key = 0;
             set_status(c.status, ST_BAD_ARG | 0x25);
-        } else if (mine < a.first || mine + a.last >= n) key = 0xffffffffu;
-        a.keys[((size_t)r * c.kvh + h) * a.stride + mine] = key;
+        } else if (b < a.first || b + a.last >= n) key = 0xffffffffu;
+        a.keys[((size_t)r * c.kvh + h) * a.stride + b] = key;
     }
 }
 
-// Block-wide exclusive prefix sum (1024 threads)
-__device__ __forceinline__ uint32_t scan_1024(uint32_t v, uint32_t *ws, uint32_t &total) {
+// Block-wide exclusive prefix sum (512 threads); two barriers
+__device__ __forceinline__ uint32_t scan_512(uint32_t v, uint32_t *ws, uint32_t &total) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= (uint32_t)o) s += t;
+        const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= (uint32_t)o) s += u;
     }
     if (lane == 31) ws[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-        uint32_t x = ws[lane];
+    uint32_t e = s - v, all = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t t = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= (uint32_t)o) x += t;
-        }
-        ws[lane] = x;
+    for (uint32_t w = 0; w < 16; w++) {
+        const uint32_t x = ws[w];
+        if (w < warp) e += x;
+        all += x;
     }
-    __syncthreads();
-    const uint32_t e = (warp ? ws[warp - 1] : 0) + s - v;
-    total = ws[31];
+    total = all;
     __syncthreads();
     return e;
 }
 
-// The `count` largest keys in ascending order of their blocks; of the keys that equal the smallest of them the lowest blocks are taken.  A thread owns a run of
-// consecutive blocks, so prefix sums give the places.  grid (kvh, nb) x 1024
-//   up to 4096 blocks: four keys per thread in registers; the threshold is found two bits at a time, one barrier each (three passes of histograms with
-//   their barriers took 8 us for 750 blocks)
-//   more: radix selection (11 + 11 + 10 bits) over the keys in memory
-__global__ void __launch_bounds__(1024) kv8_best_k(Kv8Dev c, PickArgs a) {
-    __shared__ uint32_t hist[2048], ws[32], sh_bin, sh_rem;
+// The `count` largest keys in ascending order of their blocks; of the keys that equal the smallest of them the lowest blocks are taken.  Histograms of 2048
+// equal parts of the range in play, which shrinks to the part that holds the threshold, until the threshold is found or the whole part is taken; usually two.
+// Blocks that are always taken (key 0xffffffff) and such without a page (0) are not in it.  Up to 4096 keys stay in shared memory.  In the end a thread owns
+// a run of consecutive blocks, so prefix sums give the places.  Bound: its barriers.  (Radix passes over the keys' bits, 1024 threads: 8 us for 750 blocks;
+// two bits at a time with counters: 12.)  grid (kvh, nb) x 512
+constexpr uint32_t BEST_KEYS = 4096;
+__global__ void __launch_bounds__(512) kv8_best_k(Kv8Dev c, PickArgs a) {
+    __shared__ uint32_t hist[2048], ws[16], red[16][4], found[3], kept[BEST_KEYS];
     pdl_sync();
-    const uint32_t h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    const uint32_t h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int len = a.lens[r], slot = a.slots[r];
     if (slot < 0) return;
     const bool bad = len > 0 && (uint32_t)len > a.max_len;
@@ -152,99 +142,74 @@ __global__ void __launch_bounds__(1024) kv8_best_k(Kv8Dev c, PickArgs a) {
     const uint32_t n = bad ? 0 : row_blocks(c, a, slot, len);
     const uint32_t *keys = a.keys + ((size_t)r * c.kvh + h) * a.stride;
     int32_t *out = a.out + ((size_t)r * c.kvh + h) * a.count;
-    uint32_t T = 0, rem = 0;  // keys above T are taken, and `rem` of those equal to it (T = 0: all that have a page)
-    if (n <= 4096) {
-        uint32_t k[4], at, taken = 0;
-        if (4 * tid < n) {
-            const uint4 v = __ldcg((const uint4 *)keys + tid);  // (a row's keys have room for a multiple of four)
-            k[0] = v.x, k[1] = 4 * tid + 1 < n ? v.y : 0, k[2] = 4 * tid + 2 < n ? v.z : 0, k[3] = 4 * tid + 3 < n ? v.w : 0;
-        } else k[0] = k[1] = k[2] = k[3] = 0;
-        if (n > a.count) {
-            uint32_t(*cnt)[4] = (uint32_t(*)[4])hist;
-            if (tid < 64) hist[tid] = 0;
-            __syncthreads();
-            rem = a.count;  // of the keys that share T's bits so far
-            for (int it = 0; it < 16; it++) {
-                const int sh = 30 - 2 * it;
-                // keys that share the bits above, by their next two bits: counts of 3, 2 and 1, at most 128 per warp each
-                uint32_t s = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t x = k[i] >> sh, d = x & 3;
-                    if (it == 0 || x >> 2 == T) s += d == 3 ? 1u : d == 2 ? 1u << 10 : d == 1 ? 1u << 20 : 0;
-                }
-                s = __reduce_add_sync(0xffffffffu, s);
-                if ((tid & 31) == 0 && s) {
-                    if (s & 1023) atomicAdd(&cnt[it][3], s & 1023);
-                    if (s >> 10 & 1023) atomicAdd(&cnt[it][2], s >> 10 & 1023);
-                    if (s >> 20) atomicAdd(&cnt[it][1], s >> 20);
-                }
-                __syncthreads();
-                const uint32_t c3 = cnt[it][3], c2 = cnt[it][2], c1 = cnt[it][1];
-                uint32_t d = 3;
-                if (rem > c3) {
-                    rem -= c3, d = 2;
-                    if (rem > c2) {
-                        rem -= c2, d = 1;
-                        if (rem > c1) rem -= c1, d = 0;
-                    }
-                }
-                T = T << 2 | d;
-            }
-            if (T == 0) rem = 0;  // (fewer blocks with a page than wanted)
-        }
-        uint32_t v = 0;  // taken ones above T | equal to T << 16
-#pragma unroll
-        for (int i = 0; i < 4; i++) v += k[i] > T ? 1u : T && k[i] == T ? 1u << 16 : 0;
-        const uint32_t e = scan_1024(v, ws, at);
-        uint32_t eq = e >> 16;
-        taken = (at & 0xffff) + min(at >> 16, rem);
-        uint32_t place = (e & 0xffff) + min(eq, rem);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (k[i] > T || (T && k[i] == T && eq++ < rem)) out[place++] = (int32_t)(4 * tid + i);
-        for (uint32_t i = taken + tid; i < a.count; i += 1024) out[i] = -1;
-        return;
+    uint32_t lo = 0xffffffffu, hi = 0, fixed = 0, in = 0;  // smallest, largest of the keys in play; always taken ones, ones in play
+    for (uint32_t i = tid; i < n; i += 512) {
+        const uint32_t k = __ldcg(keys + i);
+        if (i < BEST_KEYS) kept[i] = k;
+        if (k == 0xffffffffu) fixed++;
+        else if (k) lo = min(lo, k), hi = max(hi, k), in++;
     }
-    if (n > a.count) {
-        rem = a.count;
-        const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-        for (int ps = 0; ps < 3; ps++) {
-            const int sh = shifts[ps], nbins = 1 << widths[ps];
-            for (uint32_t b = tid; b < 2048; b += 1024) hist[b] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < n; i += 1024) {
-                const uint32_t key = __ldcg(keys + i);
-                if (ps == 0 || (key >> (sh + widths[ps])) == T) atomicAdd(&hist[(key >> sh) & (nbins - 1)], 1u);
+    if (n <= BEST_KEYS) keys = kept;
+    lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi), fixed = __reduce_add_sync(0xffffffffu, fixed), in = __reduce_add_sync(0xffffffffu, in);
+    if (lane == 0) red[warp][0] = lo, red[warp][1] = hi, red[warp][2] = fixed, red[warp][3] = in;
+    for (uint32_t b = tid; b < 2048; b += 512) hist[b] = 0;
+    __syncthreads();
+    lo = 0xffffffffu, hi = fixed = in = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) lo = min(lo, red[w][0]), hi = max(hi, red[w][1]), fixed += red[w][2], in += red[w][3];
+    uint32_t T = 0, rem = 0;  // keys above T are taken, and `rem` of those equal to it
+    const uint32_t want = a.count - min(a.count, fixed);
+    if (want == 0) T = 0xfffffffeu;
+    else if (in > want) {
+        rem = want;
+        for (;;) {
+            const uint32_t bits = 32 - __clz(hi - lo), sh = bits > 11 ? bits - 11 : 0;
+            for (uint32_t i = tid; i < n; i += 512) {
+                const uint32_t k = keys[i];
+                if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> sh], 1u);
             }
             __syncthreads();
-            const uint32_t b1 = 2047 - 2 * tid, b0 = b1 - 1;
-            const uint32_t h1 = b1 < (uint32_t)nbins ? hist[b1] : 0, h0 = b0 < (uint32_t)nbins ? hist[b0] : 0;
+            const uint32_t b = 2044 - 4 * tid;  // this thread's four parts
+            const uint4 v = *(const uint4 *)&hist[b];
+            *(uint4 *)&hist[b] = make_uint4(0, 0, 0, 0);
             uint32_t tot;
-            const uint32_t e = scan_1024(h1 + h0, ws, tot);  // keys in all bins above b1
-            if (e < rem && e + h1 >= rem) sh_bin = b1, sh_rem = rem - e;
-            else if (e + h1 < rem && e + h1 + h0 >= rem) sh_bin = b0, sh_rem = rem - e - h1;
+            const uint32_t e = scan_512(v.x + v.y + v.z + v.w, ws, tot);  // keys in all parts above these
+            const uint32_t cnt[4] = {v.w, v.z, v.y, v.x};
+            uint32_t at = e;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (at < rem && at + cnt[i] >= rem) found[0] = b + 3 - i, found[1] = rem - at, found[2] = cnt[i];
+                at += cnt[i];
+            }
             __syncthreads();
-            T = (T << widths[ps]) | sh_bin;
-            rem = sh_rem;
-            __syncthreads();
+            lo += found[0] << sh;
+            rem = found[1];
+            if (sh == 0) {
+                T = lo;
+                break;
+            }
+            if (found[2] == rem) {  // all of them
+                T = lo - 1;
+                rem = 0;
+                break;
+            }
+            hi = min(hi, lo + ((1u << sh) - 1));
         }
-        if (T == 0) rem = 0;
     }
-    const uint32_t run = (n + 1023) / 1024, i0 = min(n, tid * run), i1 = min(n, i0 + run);
-    uint32_t above = 0, equal = 0, tot_above, tot_equal;
+    const uint32_t run = (n + 511) / 512, i0 = min(n, tid * run), i1 = min(n, i0 + run);
+    uint32_t above = 0, equal = 0, tot_above, tot_equal = 0;
     for (uint32_t i = i0; i < i1; i++) {
-        const uint32_t key = __ldcg(keys + i);
-        above += key > T;
-        equal += T && key == T;
+        const uint32_t k = keys[i];
+        above += k > T;
+        equal += rem && k == T;
     }
-    const uint32_t ea = scan_1024(above, ws, tot_above), ee = scan_1024(equal, ws, tot_equal);
+    const uint32_t ea = scan_512(above, ws, tot_above), ee = rem ? scan_512(equal, ws, tot_equal) : 0;
     uint32_t at = ea + min(ee, rem), eq = ee;
     for (uint32_t i = i0; i < i1; i++) {
-        const uint32_t key = __ldcg(keys + i);
-        if (key > T || (T && key == T && eq++ < rem)) out[at++] = (int32_t)i;
+        const uint32_t k = keys[i];
+        if (k > T || (rem && k == T && eq++ < rem)) out[at++] = (int32_t)i;
     }
-    for (uint32_t i = tot_above + min(tot_equal, rem) + tid; i < a.count; i += 1024) out[i] = -1;
+    for (uint32_t i = tot_above + min(tot_equal, rem) + tid; i < a.count; i += 512) out[i] = -1;
 }
 
 typedef void (*pick_kernel)(Kv8Dev, PickArgs);
@@ -253,8 +218,7 @@ pick_kernel score_of(uint32_t hd, uint32_t dtype) {
     return hd == 64 ? kv8_score_k<64, __nv_bfloat16> : hd == 128 ? kv8_score_k<128, __nv_bfloat16> : kv8_score_k<256, __nv_bfloat16>;
 }
 uint32_t most_blocks(const qw_kv8_cache *c, uint32_t max_len) { return (uint32_t)(((uint64_t)max_len + c->block - 1) / c->block); }
-uint32_t key_stride(const qw_kv8_cache *c, uint32_t max_len) { return (most_blocks(c, max_len) + 3) / 4 * 4; }
-size_t work_of(const qw_kv8_cache *c, uint32_t nb, uint32_t max_len) { return (size_t)nb * c->kvh * key_stride(c, max_len) * 4; }
+size_t work_of(const qw_kv8_cache *c, uint32_t nb, uint32_t max_len) { return (size_t)nb * c->kvh * most_blocks(c, max_len) * 4; }
 int check_pick(const qw_kv8_cache *c, const qw_kv8_pick_args *a, const char **m) {
     if (!a) return *m = "no arguments", -1;
     if (!c->bounds) return *m = "the cache has no bounds", -1;
@@ -269,11 +233,11 @@ int check_pick(const qw_kv8_cache *c, const qw_kv8_pick_args *a, const char **m)
 }
 cudaError_t enqueue_pick(const qw_kv8_cache *c, const qw_kv8_pick_args *a, cudaStream_t st) {
     const uint32_t most = most_blocks(c, a->max_len);
-    const PickArgs k = {a->q, a->lens, a->slots, a->blocks, (uint32_t *)a->work, a->q_row, a->q_head, a->nb, a->qh, a->qh / c->kvh, a->max_len, a->nblocks, a->first, a->last, key_stride(c, a->max_len)};
+    const PickArgs k = {a->q, a->lens, a->slots, a->blocks, (uint32_t *)a->work, a->q_row, a->q_head, a->nb, a->qh, a->qh / c->kvh, a->max_len, a->nblocks, a->first, a->last, most};
     const Kv8Dev d = kv8_dev(c, a->layer);
     const cudaError_t e = qw_launch(score_of(c->hd, a->dtype), dim3((most + RECORDS - 1) / RECORDS, c->kvh, a->nb), 256, 0, st, d, k);
     if (e != cudaSuccess) return e;
-    return qw_launch(kv8_best_k, dim3(c->kvh, a->nb), 1024, 0, st, d, k);
+    return qw_launch(kv8_best_k, dim3(c->kvh, a->nb), 512, 0, st, d, k);
 }
 
 cudaError_t launch_kv8_pick(const QwLaunch &L) {
@@ -289,7 +253,7 @@ cudaError_t launch_kv8_pick(const QwLaunch &L) {
     return enqueue_pick(&c, &a, L.stream);
 }
 }  // namespace
-QW_FAMILY(kv8_pick, launch_kv8_pick, 1024)
+QW_FAMILY(kv8_pick, launch_kv8_pick, 512)
 
 extern "C" size_t qw_kv8_pick_work(const qw_kv8_cache *c, uint32_t nb, uint32_t max_len) {
     size_t n[3];
