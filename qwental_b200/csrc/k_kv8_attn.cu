@@ -12,8 +12,9 @@ using namespace qw;
 
 namespace {
 // Tokens of a chunk, by the tokens of its row alone (a row's result does not depend on the others of a call): short rows in small pieces, for their latency;
-// a chunk of 256 leaves 6 % of its own bytes as fp32 sums.
-__host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 8192 ? 7 : 8; }
+// a chunk of 128 leaves 12 % of its own bytes as fp32 sums, in L2.  With 256 from 8193 tokens on, one row of 48000 took 24 us instead of MEASURE1 and 16 ragged rows
+// of 1K to 48K had single warps that ended 9 us after the others.
+__host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 65536 ? 7 : 8; }
 __host__ __device__ inline uint32_t chunk_of(uint32_t n) { return 1u << chunk_log(n); }
 __host__ __device__ inline uint32_t chunks_in(uint32_t n) { return (n + chunk_of(n) - 1) >> chunk_log(n); }
 constexpr float LOWEST = 7.7037197775489434e-34f, LOWEST_LOG2 = -110.f;  // 2^-110
@@ -53,17 +54,13 @@ __device__ __forceinline__ float2 *stats_of(const AttnArgs &a, uint32_t hd, uint
     return (float2 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
 }
 
-// Four channels of a head's result: times f, times sigmoid(gate), rounded once.
-template <class T>
-__device__ __forceinline__ void finish(const AttnArgs &a, uint32_t r, uint32_t qh, uint32_t ch, float4 v, float f) {
-    float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-    if (a.gate) {
-        float g[4];
-        kv8_load<4>((const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch, g);
-#pragma unroll
-        for (int j = 0; j < 4; j++) y[j] *= 1.f / (1.f + expf(-g[j]));
-    }
-    kv8_store<4>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, y);
+// (M, l, acc) of some tokens joined with those of others
+__device__ __forceinline__ void join(float &M, float &l, float2 &acc, float M2, float l2, float2 acc2) {
+    const float m = fmaxf(M, M2), f = M == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(M - m), f2 = M2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : exp2f(M2 - m);  // (no maximum: nothing, or NaN)
+    M = m;
+    l = fmaf(l, f, l2 * f2);
+    acc.x = fmaf(acc.x, f, acc2.x * f2);
+    acc.y = fmaf(acc.y, f, acc2.y * f2);
 }
 
 // ------------------------------------------------------------------------------------------------ core
@@ -74,42 +71,47 @@ __device__ __forceinline__ void finish(const AttnArgs &a, uint32_t r, uint32_t q
 //   scores   S[16 tokens][8 heads] = codes[16][HD] . q^T     mma m16n8k16.  Which channel is which k of the product is free as long as both sides agree, so a
 //            lane takes 16 codes with one shared-memory load and they feed four products as they lie.
 //   values   O^T[16 channels][8 heads] += codes^T[16][16 tokens] . w^T     a lane takes 16 codes of four tokens; byte permutations pair the tokens; the weights
-//            change lanes by shuffles and travel as fp16 high part and remainder (22 bits).
+//            change lanes by shuffles and travel as fp16 high part and remainder (22 bits), in two products, or, of up to four heads, in the columns of one.
 // Codes become fp16 numbers exactly (kv8.cuh), queries are divided by a power of two of their own first, so the products are exact and the sums fp32.
 // Measured for 16 ragged rows of 1K to 48K tokens (210 MB, e4m3) against forms that were left: blocks of 8 warps that share a tile of 128 tokens, with two
 // barriers per tile, 87 us (scaling, maxima and barriers of a tile 2800 cycles, one after the other); e4m3 operands as they are (mma m16n8k32) no faster, that
 // product being converted to fp16 ones by the assembler at every use (19 cycles instead of 8).
 constexpr uint32_t STEP = 32;
 
-template <int HD, int NT, bool FEW>
+template <int HD, int MODE, bool FEW>
 struct Core {
+    static constexpr int NT = MODE == 2 ? 2 : 1;                        // tiles of 8 columns
+    static constexpr bool DUP = MODE == 0;                              // up to four heads: columns 4 to 7 repeat them
     static constexpr int BOX = HD < 128 ? HD : 128, HALVES = HD / BOX;  // bytes of a row in a copy, copies side by side
     static constexpr int TILE = STEP * HD;                              // K or V
     // warps that compute: what shared memory and registers (for warps in fours, the feeding one among them) allow, one block per SM
-    static constexpr int WARPS = FEW ? 4 : HD == 256 ? (NT == 1 ? 11 : 7) : NT == 1 ? 12 : 11;
-    static constexpr int RING = (FEW ? 3 : 1) * 256 / HD;               // tiles of either: 16 KB per warp, or 48
+    static constexpr int WARPS = FEW ? 4 : HD == 256 ? (NT == 1 ? 11 : 7) : NT == 1 ? 15 : 11;
+    static constexpr int KR = FEW ? 3 * 256 / HD : HD == 256 ? 1 : HD == 128 ? 2 : NT == 1 ? 3 : 4;  // K and V tiles of a warp: 12 to 16 KB, or 48
+    static constexpr int VR = FEW ? KR : HD == 256 ? 1 : HD == 128 ? (NT == 1 ? 1 : 2) : NT == 1 ? 3 : 4;
     static constexpr int CH = HALVES * (HD < 128 ? 4 : 8);              // 16-channel tiles
     static constexpr int LANE = HD < 128 ? 8 : 16;                      // channels of a lane in a row of a copy
-    static constexpr int SLOTS = WARPS * RING, THREADS = 32 * (WARPS + 1);
+    static constexpr int THREADS = 32 * (WARPS + 1);
     // shared memory behind the tiles: scales of K and V, what a tile is, mbarriers (full and empty, K and V); then 12 bytes per row
-    static constexpr int SCALES = SLOTS * 2 * TILE, INFO = SCALES + SLOTS * 2 * STEP * 4, BARS = INFO + SLOTS * 32, HAS = BARS + SLOTS * 32, ROWS = HAS + 64, BYTES = ROWS + 1024 + 16;
+    static constexpr int SCALES = WARPS * (KR + VR) * TILE, INFO = SCALES + WARPS * KR * 2 * STEP * 4, BARS = INFO + WARPS * KR * 32, HAS = BARS + WARPS * (KR + VR) * 16,
+                         ROWS = HAS + 64, BYTES = ROWS + 1024 + 16;
     static_assert(WARPS + 1 <= 16 && BYTES + 12 * KV8_MAX_ROWS <= 227 * 1024, "words of HAS, and what a block may have");
 };
 
-template <int HD, int FMT, class T, int NT, bool FEW>
-__global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
-    typedef Core<HD, NT, FEW> X;
-    constexpr int RING = X::RING;
+template <int HD, int FMT, class T, int MODE, bool FEW>
+__global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
+    typedef Core<HD, MODE, FEW> X;
+    constexpr int KR = X::KR, VR = X::VR, NT = X::NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // swizzled copies need it
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     uint32_t *has = (uint32_t *)(smem + X::HAS), *first = (uint32_t *)(smem + X::ROWS), *lenv = first + a.nb + 1, *slotv = lenv + a.nb;
     // of warp w: its K tiles, then its V tiles; full and empty barriers of both
-    auto tiles_of = [&](uint32_t w) { return smem_u32(smem) + w * RING * 2 * X::TILE; };
-    auto scales_of = [&](uint32_t w) { return (float *)(smem + X::SCALES) + w * RING * 2 * STEP; };
-    auto info_of = [&](uint32_t w) { return (uint4 *)(smem + X::INFO) + w * RING * 2; };
-    auto bars_of = [&](uint32_t w) { return (uint64_t *)(smem + X::BARS) + w * RING * 4; };
-    for (uint32_t i = tid; i < X::SLOTS * 4; i += X::THREADS) mbar_init((uint64_t *)(smem + X::BARS) + i, 1);
+    auto tiles_of = [&](uint32_t w) { return smem_u32(smem) + w * (KR + VR) * X::TILE; };
+    auto scales_of = [&](uint32_t w) { return (float *)(smem + X::SCALES) + w * KR * 2 * STEP; };
+    auto info_of = [&](uint32_t w) { return (uint4 *)(smem + X::INFO) + w * KR * 2; };
+    auto bars_of = [&](uint32_t w) { return (uint64_t *)(smem + X::BARS) + w * (KR + VR) * 2; };
+    constexpr int KF = 0, VF = KR, KE = KR + VR, VE = 2 * KR + VR;
+    for (uint32_t i = tid; i < X::WARPS * (KR + VR) * 2; i += X::THREADS) mbar_init((uint64_t *)(smem + X::BARS) + i, 1);
     mbar_init_fence();
     __syncthreads();
     pdl_sync();
@@ -172,7 +174,8 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         f.at = f.r < a.nb ? first[f.r] * c.kvh + f.h * f.steps + f.ch * f.cs : total;
     };
     auto find = [&](uint32_t w) {  // warp w's; returns the end of its share
-        const uint32_t W = gridDim.x * X::WARPS, w0 = w * gridDim.x + blockIdx.x;  // (few tasks go to different SMs first)
+        // few tasks go to different SMs first; many to neighbours, who mostly read the same queries
+        const uint32_t W = gridDim.x * X::WARPS, w0 = FEW ? w * gridDim.x + blockIdx.x : blockIdx.x * X::WARPS + w;
         const uint32_t lo = (uint32_t)((uint64_t)w0 * total / W), hi = (uint32_t)((uint64_t)(w0 + 1) * total / W);
         f.at = total;
         if (lo < hi) {
@@ -232,14 +235,14 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         uint64_t *bars = bars_of(lane < X::WARPS ? lane : 0);
         uint4 *info = info_of(lane < X::WARPS ? lane : 0);
         float *scales = scales_of(lane < X::WARPS ? lane : 0);
-        const uint32_t Kt = tiles_of(lane < X::WARPS ? lane : 0), Vt = Kt + RING * X::TILE, vrows = c.kvh * KV8_PAGE;
+        const uint32_t Kt = tiles_of(lane < X::WARPS ? lane : 0), Vt = Kt + KR * X::TILE, vrows = c.kvh * KV8_PAGE;
         uint32_t fed = 0, vfed = 0;  // K and V tiles so far
         uint64_t t0 = global_ns();
         bool ok = true;
         while (__any_sync(0xffffffffu, more || vfed < fed)) {
             bool did = false;
-            const uint32_t sl = fed % RING, vl = vfed % RING;
-            if (more && fed < vfed + RING /* V of the tile whose place it takes has gone */ && (fed < RING || mbar_test(&bars[2 * RING + sl], fed / RING - 1 & 1))) {
+            const uint32_t sl = fed % KR, vl = vfed % VR;
+            if (more && fed < vfed + KR /* V of the tile whose place it takes has gone */ && (fed < KR || mbar_test(&bars[KE + sl], fed / KR - 1 & 1))) {
                 uint32_t row[2] = {0, 0};
 #pragma unroll
                 for (int e = 0; e < 2; e++)
@@ -259,29 +262,29 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                     more = f.at < hi;
                 }
                 info[2 * sl + 1] = make_uint4(r, h, ch, of | (more ? 0u : 4u));
-                mbar_expect_tx(&bars[sl], (on0 + on1) * box_rows * (HD + 8));
+                mbar_expect_tx(&bars[KF + sl], (on0 + on1) * box_rows * (HD + 8));
 #pragma unroll
                 for (int e = 0; e < 2; e++)
                     if (e ? on1 : on0) {
                         float *sc = scales + sl * 2 * STEP + e * 16;
 #pragma unroll
-                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kt + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row[e], &bars[sl]);
-                        bulk_g2s(sc, c.scales + row[e], box_rows * 4, &bars[sl]);
-                        bulk_g2s(sc + STEP, c.scales + row[e] + vrows, box_rows * 4, &bars[sl]);
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kt + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row[e], &bars[KF + sl]);
+                        bulk_g2s(sc, c.scales + row[e], box_rows * 4, &bars[KF + sl]);
+                        bulk_g2s(sc + STEP, c.scales + row[e] + vrows, box_rows * 4, &bars[KF + sl]);
                     }
                 fed++;
                 if (more) ask();
                 did = true;
             }
-            if (vfed < fed && (vfed < RING || mbar_test(&bars[3 * RING + vl], vfed / RING - 1 & 1))) {
-                const uint4 v = info[2 * vl];
+            if (vfed < fed && (vfed < VR || mbar_test(&bars[VE + vl], vfed / VR - 1 & 1))) {
+                const uint4 v = info[2 * (vfed % KR)];
                 const bool on0 = v.x && !(v.x >> 16), on1 = box_rows == 16 && v.y && !(v.y >> 16);
-                mbar_expect_tx(&bars[RING + vl], (on0 + on1) * box_rows * HD);
+                mbar_expect_tx(&bars[VF + vl], (on0 + on1) * box_rows * HD);
 #pragma unroll
                 for (int e = 0; e < 2; e++)
                     if (e ? on1 : on0) {
 #pragma unroll
-                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? v.w : v.z) + vrows), &bars[RING + vl]);
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? v.w : v.z) + vrows), &bars[VF + vl]);
                     }
                 vfed++;
                 did = true;
@@ -294,8 +297,8 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
         }
         if (!ok) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
             if (lane == 0) set_status(status, ST_MBAR_TIMEOUT | 0x23);
-            for (uint32_t x = fed < RING ? 0 : fed - RING; x < fed; x++) mbar_wait(&bars[x % RING], x / RING & 1);
-            for (uint32_t x = vfed < RING ? 0 : vfed - RING; x < vfed; x++) mbar_wait(&bars[RING + x % RING], x / RING & 1);
+            for (uint32_t x = fed < KR ? 0 : fed - KR; x < fed; x++) mbar_wait(&bars[KF + x % KR], x / KR & 1);
+            for (uint32_t x = vfed < VR ? 0 : vfed - VR; x < vfed; x++) mbar_wait(&bars[VF + x % VR], x / VR & 1);
         }
         return;
     }
@@ -307,14 +310,14 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
     uint32_t n = 0, have_r = 0xffffffffu, have_h = 0;
     uint32_t qf[NT][HD / 8];
     float fac[NT][2], o[X::CH][NT][4], M[NT][2], l[NT][2];
-    const uint32_t Kb = tiles_of(warp), Vb = Kb + RING * X::TILE;
+    const uint32_t Kb = tiles_of(warp), Vb = Kb + KR * X::TILE;
     uint64_t *bars = bars_of(warp);
     auto load_queries = [&](uint32_t r, uint32_t h) {
         // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
         have_r = r, have_h = h;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const uint32_t head = nt * 8 + g;
+            const uint32_t head = X::DUP ? g & 3 : nt * 8 + g;
             const T *qp = (const T *)a.q + (int64_t)r * a.q_row + (int64_t)(h * a.G + min(head, a.G - 1)) * a.q_head;
             uint32_t m = 0;
 #pragma unroll
@@ -349,8 +352,8 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
     };
     load_queries(f.r, f.h);  // the first task's, while its tile is on its way
     for (; more; n++) {
-        const uint32_t sl = n % RING;
-        if (!mbar_wait(&bars[sl], n / RING & 1)) {
+        const uint32_t sl = n % KR, vl = n % VR;
+        if (!mbar_wait(&bars[KF + sl], n / KR & 1)) {
             ok = false;
             break;
         }
@@ -416,7 +419,7 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                     }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[2 * RING + sl]);
+            if (lane == 0) mbar_arrive(&bars[KE + sl]);
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
@@ -483,9 +486,10 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                     const uint32_t x = *(const uint32_t *)&h;
                     return __byte_perm(__shfl_sync(0xffffffffu, x, srcA), __shfl_sync(0xffffffffu, x, srcB), sel);
                 };
-                p[mt][nt][0] = to_b(h01), p[mt][nt][1] = to_b(h23), p[mt][nt][2] = to_b(r01), p[mt][nt][3] = to_b(r23);
+                if (X::DUP) p[mt][nt][0] = to_b(t < 2 ? h01 : r01), p[mt][nt][1] = to_b(t < 2 ? h23 : r23);  // columns 4 to 7 are the same heads: their remainders
+                else p[mt][nt][0] = to_b(h01), p[mt][nt][1] = to_b(h23), p[mt][nt][2] = to_b(r01), p[mt][nt][3] = to_b(r23);
             }
-        if (!mbar_wait(&bars[RING + sl], n / RING & 1)) {
+        if (!mbar_wait(&bars[VF + vl], n / VR & 1)) {
             ok = false;
             break;
         }
@@ -498,8 +502,8 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t row = mt * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
-                    if (HD == 64) lds64(w[e][0], w[e][1], Vb + sl * X::TILE + row * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8);
-                    else lds128(w[e], Vb + sl * X::TILE + hf * STEP * 128 + row * 128 + ((g ^ (2 * t + (e & 1))) << 4));
+                    if (HD == 64) lds64(w[e][0], w[e][1], Vb + vl * X::TILE + row * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8);
+                    else lds128(w[e], Vb + vl * X::TILE + hf * STEP * 128 + row * 128 + ((g ^ (2 * t + (e & 1))) << 4));
                 }
                 if (cnt[mt] < 16) {  // rows behind the last token may hold anything, and 0 times a code that is no number would reach every head
 #pragma unroll
@@ -518,17 +522,25 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
                         float(&y0)[4] = o[hf * 8 + 2 * x][nt], (&y1)[4] = o[hf * 8 + 2 * x + 1][nt];
                         mma_f16(y0, a0, p[mt][nt][0], p[mt][nt][1], y0);
                         mma_f16(y1, a1, p[mt][nt][0], p[mt][nt][1], y1);
-                        mma_f16(y0, a0, p[mt][nt][2], p[mt][nt][3], y0);
-                        mma_f16(y1, a1, p[mt][nt][2], p[mt][nt][3], y1);
+                        if (!X::DUP) {
+                            mma_f16(y0, a0, p[mt][nt][2], p[mt][nt][3], y0);
+                            mma_f16(y1, a1, p[mt][nt][2], p[mt][nt][3], y1);
+                        }
                     }
                 }
             }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[3 * RING + sl]);
+        if (lane == 0) mbar_arrive(&bars[VE + vl]);
         if (task.w & 2) {  // ---- the chunk's totals
             const size_t at = (size_t)task.x * a.max_chunks + task.z;
             float *dst = a.part + (at * a.qh + task.y * a.G + 2 * t) * HD + X::LANE * g;
             float2 *st = stats_of(a, HD, task.x, task.y * a.G + 2 * t) + task.z;
+            if (X::DUP) {
+#pragma unroll
+                for (int x = 0; x < X::CH; x++)
+#pragma unroll
+                    for (int z = 0; z < 4; z++) o[x][0][z] += __shfl_xor_sync(0xffffffffu, o[x][0][z], 2);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -552,33 +564,54 @@ __global__ void __launch_bounds__(Core<HD, NT, FEW>::THREADS, 1) kv8_attn_k(cons
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Up to 32 chunks: a warp per 64 channels of a (head, row), two channels and one chunk's weight per lane; every load leaves before the weights are known.
-// The operations of a row are those of kv8_merge_k in the same order.  (Rows of length 0 get their zeros here.)  grid ceil(nb qh hd / 512) x 256
-template <int HD, class T>
-__global__ void __launch_bounds__(256) kv8_merge_few_k(Kv8Dev c, AttnArgs a) {
+// 64 channels of a (head, row): two channels per lane.  A warp takes 32 chunks at a time, a lane knows one chunk's weight (within the 32: relative to their
+// maximum) and every load leaves before the weights are known; the 32 are added in order, then joined with what the warp has.  W warps take every Wth 32 and are
+// joined in order, so a row's result depends on its own chunks alone, and up to 32 chunks W does not matter.  Rows of length 0 get their zeros here.
+// Bound: the latency of a few loads one after the other.  W = 1 for calls of up to 32 chunks (4096 (head, row) pairs of 32 chunks: 16 us in blocks of 256 threads
+// per 64 channels, 7 this way), W = 4 for longer ones.  grid (8 / W) (head, row, 64 channels) per block of 256 (W = 1) or 1 per block of 128
+template <int HD, class T, int W>
+__global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, AttnArgs a) {
+    __shared__ float2 part[W][32], stat[W];
     pdl_sync();
-    const uint32_t x = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, ch = x % (HD / 64) * 64 + 2 * lane, y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = W == 1 ? blockIdx.x * 8 + warp : blockIdx.x;
+    const uint32_t ch = x % (HD / 64) * 64 + 2 * lane, y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
     if (r >= a.nb) return;
     const int len = a.lens[r], slot = a.slots[r];
     if (slot < 0) return;
     const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
-    const float2 st = lane < nch ? __ldcg(stats_of(a, HD, r, qh) + lane) : make_float2(-INFINITY, 0.f);
+    const float2 *st = stats_of(a, HD, r, qh);
     const float *p = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch;
     const uint32_t cs = a.qh * HD;
     float2 gate = make_float2(0.f, 0.f);
-    const T *gp = (const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch;
-    if (a.gate) gate = make_float2(kv8_float(gp[0]), kv8_float(gp[1]));
-    float2 v[32];
-#pragma unroll
-    for (uint32_t k = 0; k < 32; k++) v[k] = k < nch ? __ldcg((const float2 *)(p + (size_t)k * cs)) : make_float2(0.f, 0.f);
-    const float M = warp_max(st.x), w = st.x == -INFINITY ? 0.f : exp2f(st.x - M);
-    const float l = warp_sum(st.x == -INFINITY ? st.y : st.y * w);  // (0, or NaN, where a chunk has no maximum)
+    if (a.gate && warp % W == 0) {
+        const T *gp = (const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch;
+        gate = make_float2(kv8_float(gp[0]), kv8_float(gp[1]));
+    }
+    float M = -INFINITY, l = 0.f;
     float2 acc = make_float2(0.f, 0.f);
+    for (uint32_t k0 = W == 1 ? 0 : 32 * warp; k0 < nch; k0 += 32 * W) {
+        const float2 s = k0 + lane < nch ? __ldcg(st + k0 + lane) : make_float2(-INFINITY, 0.f);
+        float2 v[32];
 #pragma unroll
-    for (uint32_t k = 0; k < 16; k++) {
-        const float w0 = __shfl_sync(0xffffffffu, w, k), w1 = __shfl_sync(0xffffffffu, w, k + 16);
-        acc.x += fmaf(v[k + 16].x, w1, __fmul_rn(v[k].x, w0));
-        acc.y += fmaf(v[k + 16].y, w1, __fmul_rn(v[k].y, w0));
+        for (uint32_t k = 0; k < 32; k++) v[k] = k0 + k < nch ? __ldcg((const float2 *)(p + (size_t)(k0 + k) * cs)) : make_float2(0.f, 0.f);
+        const float Mb = warp_max(s.x), w = s.x == -INFINITY ? 0.f : exp2f(s.x - Mb);
+        const float lb = warp_sum(s.x == -INFINITY ? s.y : s.y * w);  // (0, or NaN, where a chunk has no maximum)
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (uint32_t k = 0; k < 32; k++) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            sum.x = __fadd_rn(sum.x, __fmul_rn(v[k].x, wk));
+            sum.y = __fadd_rn(sum.y, __fmul_rn(v[k].y, wk));
+        }
+        join(M, l, acc, Mb, lb, sum);
+    }
+    if (W > 1) {
+        part[warp % W][lane] = acc;
+        if (lane == 0) stat[warp % W] = make_float2(M, l);
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int i = 1; i < W; i++) join(M, l, acc, stat[i].x, stat[i].y, part[i][lane]);
     }
     const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
@@ -588,96 +621,30 @@ __global__ void __launch_bounds__(256) kv8_merge_few_k(Kv8Dev c, AttnArgs a) {
     kv8_store<2>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, out);
 }
 
-// More: a block per 64 channels of a (head, row): 16 threads take four channels each of every 16th chunk, the 16 sums are added in order.  The first eight loads
-// of a thread leave before the weights are known.  (A first form with a block per head went through 188 chunks, 48000 tokens, in 47 dependent rounds: 30 us.)
-// grid (qh hd / 64, nb) x 256
-template <int HD, class T>
-__global__ void __launch_bounds__(256) kv8_merge_k(Kv8Dev c, AttnArgs a) {
-    __shared__ float4 accs[16][16];
-    __shared__ float wm[8], wl[8];
-    pdl_sync();
-    const uint32_t qh = blockIdx.x / (HD / 64), ch = blockIdx.x % (HD / 64) * 64, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % 16, cg = tid / 16;
-    const int len = a.lens[r], slot = a.slots[r];
-    if (slot < 0) return;
-    const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
-    const float2 *st = stats_of(a, HD, r, qh);
-    const float4 *p = (const float4 *)(a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch) + wc;
-    const size_t cs = (size_t)a.qh * (HD / 4);
-    float4 v[8];
-    float Mv[8];
-    auto load = [&](uint32_t k0) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t k = k0 + 16 * i;
-            Mv[i] = k < nch ? __ldcg(&st[k].x) : -INFINITY;
-            v[i] = k < nch ? __ldcg(p + k * cs) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    };
-    load(cg);
-    float M = -INFINITY;
-    for (uint32_t k = tid; k < nch; k += 256) M = fmaxf(M, __ldcg(&st[k].x));
-    M = warp_max(M);
-    if (lane == 0) wm[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) M = fmaxf(M, wm[w]);
-    float l = 0.f;
-    for (uint32_t k = tid; k < nch; k += 256) {
-        const float2 s = __ldcg(st + k);
-        l += s.x == -INFINITY ? s.y : s.y * exp2f(s.x - M);  // (0, or NaN, where a chunk has no maximum)
-    }
-    l = warp_sum(l);
-    if (lane == 0) wl[warp] = l;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t k0 = cg; k0 < nch;) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float w = Mv[i] == -INFINITY ? 0.f : exp2f(Mv[i] - M);
-            acc.x = fmaf(v[i].x, w, acc.x), acc.y = fmaf(v[i].y, w, acc.y), acc.z = fmaf(v[i].z, w, acc.z), acc.w = fmaf(v[i].w, w, acc.w);
-        }
-        k0 += 128;
-        if (k0 < nch) load(k0);
-    }
-    accs[cg][wc] = acc;
-    __syncthreads();
-    if (tid >= 16) return;
-    l = wl[0];
-#pragma unroll
-    for (int w = 1; w < 8; w++) l += wl[w];
-#pragma unroll
-    for (int g = 1; g < 16; g++) {
-        const float4 u = accs[g][tid];
-        acc.x += u.x, acc.y += u.y, acc.z += u.z, acc.w += u.w;
-    }
-    const bool bad = len > 0 && (uint32_t)len > a.max_len;
-    if (bad && tid == 0) set_status(c.status, ST_BAD_ARG | 0x24);
-    finish<T>(a, r, qh, ch + 4 * tid, acc, bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l);
-}
-
 // Which kernel: by the format, the type of rows, and whether 8 or 16 heads share a kv head.
 typedef void (*core_kernel)(CUtensorMap, Kv8Dev, AttnArgs, uint32_t, unsigned *);
 typedef void (*merge_kernel)(Kv8Dev, AttnArgs);
 struct Launch {
     core_kernel core;
-    merge_kernel merge, merge_few;
+    merge_kernel merge, merge_few;  // of more than 32 chunks, of up to 32
     int smem, threads;  // shared memory but for 12 bytes per row
 };
-template <int HD, int FMT, class T, int NT, bool FEW>
+template <int HD, int FMT, class T, int MODE, bool FEW>
 Launch launch_of() {
-    return {kv8_attn_k<HD, FMT, T, NT, FEW>, kv8_merge_k<HD, T>, kv8_merge_few_k<HD, T>, Core<HD, NT, FEW>::BYTES, Core<HD, NT, FEW>::THREADS};
+    return {kv8_attn_k<HD, FMT, T, MODE, FEW>, kv8_merge_k<HD, T, 4>, kv8_merge_k<HD, T, 1>, Core<HD, MODE, FEW>::BYTES, Core<HD, MODE, FEW>::THREADS};
 }
 template <int HD, int FMT, class T>
-Launch launch_of(bool wide, bool few) {
-    if (few) return wide ? launch_of<HD, FMT, T, 2, true>() : launch_of<HD, FMT, T, 1, true>();
-    return wide ? launch_of<HD, FMT, T, 2, false>() : launch_of<HD, FMT, T, 1, false>();
+Launch launch_of(uint32_t G, bool few) {
+    if (few) return G > 8 ? launch_of<HD, FMT, T, 2, true>() : G > 4 ? launch_of<HD, FMT, T, 1, true>() : launch_of<HD, FMT, T, 0, true>();
+    return G > 8 ? launch_of<HD, FMT, T, 2, false>() : G > 4 ? launch_of<HD, FMT, T, 1, false>() : launch_of<HD, FMT, T, 0, false>();
 }
 template <int HD>
-Launch launch_of(uint32_t format, uint32_t dtype, bool wide, bool few) {
-    if (format == QW_KV8_E4M3) return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_E4M3, __half>(wide, few) : launch_of<HD, QW_KV8_E4M3, __nv_bfloat16>(wide, few);
-    return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_INT8, __half>(wide, few) : launch_of<HD, QW_KV8_INT8, __nv_bfloat16>(wide, few);
+Launch launch_of(uint32_t format, uint32_t dtype, uint32_t G, bool few) {
+    if (format == QW_KV8_E4M3) return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_E4M3, __half>(G, few) : launch_of<HD, QW_KV8_E4M3, __nv_bfloat16>(G, few);
+    return dtype == QW_KV8_FP16 ? launch_of<HD, QW_KV8_INT8, __half>(G, few) : launch_of<HD, QW_KV8_INT8, __nv_bfloat16>(G, few);
 }
-Launch launch_of(uint32_t hd, uint32_t format, uint32_t dtype, bool wide, bool few) {
-    return hd == 64 ? launch_of<64>(format, dtype, wide, few) : hd == 128 ? launch_of<128>(format, dtype, wide, few) : launch_of<256>(format, dtype, wide, few);
+Launch launch_of(uint32_t hd, uint32_t format, uint32_t dtype, uint32_t G, bool few) {
+    return hd == 64 ? launch_of<64>(format, dtype, G, few) : hd == 128 ? launch_of<128>(format, dtype, G, few) : launch_of<256>(format, dtype, G, few);
 }
 
 uint32_t chunks_of(const qw_kv8_cache *c, uint32_t max_len, uint32_t nblocks) {
@@ -686,7 +653,7 @@ uint32_t chunks_of(const qw_kv8_cache *c, uint32_t max_len, uint32_t nblocks) {
     // the most chunks of a row of up to n tokens: a longer row may have fewer, at the steps of chunk_of
     const uint32_t m = (uint32_t)(n < 0xffffff00u ? n : 0xffffff00u);
     uint32_t most = chunks_in(m);
-    for (uint32_t e : {512u, 2048u, 8192u})
+    for (uint32_t e : {512u, 2048u, 65536u})
         if (e < m && chunks_in(e) > most) most = chunks_in(e);
     return most;
 }
@@ -723,15 +690,15 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
                  c->hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
     const uint64_t most = (uint64_t)a->nb * mc * c->kvh, sms = (uint64_t)kv8_sm_count();
-    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G > 8, most <= 4 * sms);
+    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G, most <= 4 * sms);
     const int smem = L.smem + (int)a->nb * 12;
     cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     e = qw_launch(L.core, (uint32_t)(most < sms ? most : sms), L.threads, smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess) return e;
-    // 4096 (head, row) pairs of 32 chunks took 16 us in blocks of 64 channels
-    if (mc <= 32) return qw_launch(L.merge_few, (uint32_t)(((uint64_t)a->nb * a->qh * (c->hd / 64) + 7) / 8), 256, 0, st, d, k);
-    return qw_launch(L.merge, dim3(a->qh * (c->hd / 64), a->nb), 256, 0, st, d, k);
+    const uint32_t units = a->nb * a->qh * (c->hd / 64);  // (at most 2^28)
+    if (mc <= 32) return qw_launch(L.merge_few, (units + 7) / 8, 256, 0, st, d, k);
+    return qw_launch(L.merge, units, 128, 0, st, d, k);
 }
 
 cudaError_t launch_kv8_attn(const QwLaunch &L) {
