@@ -85,8 +85,8 @@ struct Core {
     static constexpr int BOX = HD < 128 ? HD : 128, HALVES = HD / BOX;  // bytes of a row in a copy, copies side by side
     static constexpr int TILE = STEP * HD;                              // K or V
     // warps that compute: what shared memory and registers (for warps in fours, the feeding one among them) allow, one block per SM
-    static constexpr int WARPS = FEW ? 4 : HD == 256 ? (NT == 1 ? 11 : 7) : NT == 1 ? 15 : 11;
-    static constexpr int KR = FEW ? 3 * 256 / HD : HD == 256 ? 1 : HD == 128 ? 2 : NT == 1 ? 3 : 4;  // K and V tiles of a warp: 12 to 16 KB, or 48
+    static constexpr int WARPS = FEW ? 6 : HD == 256 ? (NT == 1 ? 11 : 7) : NT == 1 ? 15 : 11;
+    static constexpr int KR = FEW ? 2 * 256 / HD : HD == 256 ? 1 : HD == 128 ? 2 : NT == 1 ? 3 : 4;  // K and V tiles of a warp: 12 to 16 KB, or 32
     static constexpr int VR = FEW ? KR : HD == 256 ? 1 : HD == 128 ? (NT == 1 ? 1 : 2) : NT == 1 ? 3 : 4;
     static constexpr int CH = HALVES * (HD < 128 ? 4 : 8);              // 16-channel tiles
     static constexpr int LANE = HD < 128 ? 8 : 16;                      // channels of a lane in a row of a copy
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
     auto find = [&](uint32_t w) {  // warp w's; returns the end of its share
         // few tasks go to different SMs first; many to neighbours, who mostly read the same queries
         const uint32_t W = gridDim.x * X::WARPS, w0 = FEW ? w * gridDim.x + blockIdx.x : blockIdx.x * X::WARPS + w;
-        const uint32_t lo = (uint32_t)((uint64_t)w0 * total / W), hi = (uint32_t)((uint64_t)(w0 + 1) * total / W);
+        const uint32_t per = total / W, rest = total - per * W, lo = w0 * per + w0 * rest / W, hi = (w0 + 1) * per + (w0 + 1) * rest / W;  // (total w / W, in 32 bits)
         f.at = total;
         if (lo < hi) {
             uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
@@ -237,7 +237,9 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
         float *scales = scales_of(lane < X::WARPS ? lane : 0);
         const uint32_t Kt = tiles_of(lane < X::WARPS ? lane : 0), Vt = Kt + KR * X::TILE, vrows = c.kvh * KV8_PAGE;
         uint32_t fed = 0, vfed = 0;  // K and V tiles so far
-        uint64_t t0 = global_ns();
+        const uint64_t once = evict_first_policy();
+        uint64_t t0 = 0;
+        uint32_t idle = 0;
         bool ok = true;
         while (__any_sync(0xffffffffu, more || vfed < fed)) {
             bool did = false;
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                     if (e ? on1 : on0) {
                         float *sc = scales + sl * 2 * STEP + e * 16;
 #pragma unroll
-                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Kt + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row[e], &bars[KF + sl]);
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d_hint(Kt + sl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)row[e], &bars[KF + sl], once);
                         bulk_g2s(sc, c.scales + row[e], box_rows * 4, &bars[KF + sl]);
                         bulk_g2s(sc + STEP, c.scales + row[e] + vrows, box_rows * 4, &bars[KF + sl]);
                     }
@@ -284,15 +286,18 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 for (int e = 0; e < 2; e++)
                     if (e ? on1 : on0) {
 #pragma unroll
-                        for (int d = 0; d < X::HALVES; d++) tma_load_2d(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? v.w : v.z) + vrows), &bars[VF + vl]);
+                        for (int d = 0; d < X::HALVES; d++) tma_load_2d_hint(Vt + vl * X::TILE + d * STEP * 128 + e * 16 * X::BOX, &tm, d * 128, (int)((e ? v.w : v.z) + vrows), &bars[VF + vl], once);
                     }
                 vfed++;
                 did = true;
             }
-            if (__any_sync(0xffffffffu, did)) t0 = global_ns();
-            else if (__any_sync(0xffffffffu, global_ns() - t0 > 2000000000ull)) {
-                ok = false;
-                break;
+            if (__any_sync(0xffffffffu, did)) idle = 0;
+            else if ((++idle & 255) == 0) {  // a wait of two seconds is given up
+                if (idle == 256) t0 = global_ns();
+                else if (__any_sync(0xffffffffu, global_ns() - t0 > 2000000000ull)) {
+                    ok = false;
+                    break;
+                }
             }
         }
         if (!ok) {  // no block ends with copies of its own in flight: those that may be are waited for, with a limit again
@@ -690,7 +695,7 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
                  c->hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
     const uint64_t most = (uint64_t)a->nb * mc * c->kvh, sms = (uint64_t)kv8_sm_count();
-    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G, most <= 4 * sms);
+    const Launch L = launch_of(c->hd, c->format, a->dtype, k.G, most <= 6 * sms);
     const int smem = L.smem + (int)a->nb * 12;
     cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;

@@ -107,11 +107,11 @@ template <class T>
 __device__ __forceinline__ void kv8_load_raw8(const T *p, uint32_t (&w)[4]) {
     const uint16_t *u = (const uint16_t *)p;
     if (((uintptr_t)p & 15) == 0) {
-        const uint4 v = __ldcg((const uint4 *)p);
+        const uint4 v = *(const uint4 *)p;  // (through L1: the warps of a block mostly want the same)
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = (uint32_t)__ldcg(u + 2 * i) | (uint32_t)__ldcg(u + 2 * i + 1) << 16;
+        for (int i = 0; i < 4; i++) w[i] = (uint32_t)u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
     }
 }
 template <class T>
