@@ -17,8 +17,32 @@ struct RowArgs {
 };
 
 // ------------------------------------------------------------------------------------------------ rows in
-// A warp per (row, head, K or V); a lane holds hd / 32 consecutive values.  Bound: 6 bytes per value pass, 3.1 MB for 1024 rows of the benchmark's layer.
-// grid nb x 256
+// One row of one head into row number `row` of the cache, by a warp; a lane holds hd / 32 consecutive values.
+template <int HD, int FMT>
+__device__ __forceinline__ void quantise_row(const Kv8Dev &c, size_t row, const float (&x)[HD / 32]) {
+    constexpr int E = HD / 32;
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t m = 0;  // largest magnitude as bits: a NaN is above the infinities, those above all numbers
+#pragma unroll
+    for (int i = 0; i < E; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    const float am = __uint_as_float(m), F = kv8_largest<FMT>();
+    const bool nan = m >= 0x7f800000u, zero = !nan && am < KV8_TINY;
+    const float inv = nan || zero ? 0.f : __fdiv_rn(F, am);
+    uint32_t w[(E + 3) / 4] = {};
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        const float y0 = nan ? 0.f : fminf(fmaxf(__fmul_rn(x[i], inv), -F), F), y1 = nan ? 0.f : fminf(fmaxf(__fmul_rn(x[i + 1], inv), -F), F);
+        w[i / 4] |= kv8_encode2<FMT>(y0, y1) << (i % 4 * 8);
+    }
+    uint8_t *dst = c.codes + row * HD + lane * E;
+    if (E == 8) *(uint2 *)dst = make_uint2(w[0], w[E == 8 ? 1 : 0]);
+    else if (E == 4) *(uint32_t *)dst = w[0];
+    else *(uint16_t *)dst = (uint16_t)w[0];
+    if (lane == 0) c.scales[row] = nan ? __uint_as_float(0x7fffffffu) : zero ? 0.f : __fdiv_rn(am, F);
+}
+
+// A cache without bounds: a warp per (row, head, K or V).  Bound: 6 bytes per value pass, 3.1 MB for 1024 rows of the benchmark's layer.  grid nb x 256
 template <int HD, int FMT, class T>
 __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
     constexpr int E = HD / 32;
@@ -36,95 +60,109 @@ __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
     if (__syncthreads_or(later)) return;
     for (uint32_t t = warp; t < 2 * c.kvh; t += 8) {
         const uint32_t kv = t >= c.kvh, h = t - kv * c.kvh;
-        const T *src = (const T *)(kv ? a.v : a.k) + (int64_t)r * (kv ? a.v_row : a.k_row) + (int64_t)h * (kv ? a.v_head : a.k_head) + lane * E;
         float x[E];
-        kv8_load<E>(src, x);
-        uint32_t m = 0;  // largest magnitude as bits: a NaN is above the infinities, those above all numbers
-#pragma unroll
-        for (int i = 0; i < E; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-        m = __reduce_max_sync(0xffffffffu, m);
-        const float am = __uint_as_float(m), F = kv8_largest<FMT>();
-        const bool nan = m >= 0x7f800000u, zero = !nan && am < KV8_TINY;
-        const float inv = nan || zero ? 0.f : __fdiv_rn(F, am);
-        uint32_t w[(E + 3) / 4] = {};
-#pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const float y0 = nan ? 0.f : fminf(fmaxf(__fmul_rn(x[i], inv), -F), F), y1 = nan ? 0.f : fminf(fmaxf(__fmul_rn(x[i + 1], inv), -F), F);
-            w[i / 4] |= kv8_encode2<FMT>(y0, y1) << (i % 4 * 8);
-        }
-        const size_t row = (size_t)kv8_row0(c, page, kv, h) + pos % KV8_PAGE;
-        uint8_t *dst = c.codes + row * HD + lane * E;
-        if (E == 8) *(uint2 *)dst = make_uint2(w[0], w[E == 8 ? 1 : 0]);
-        else if (E == 4) *(uint32_t *)dst = w[0];
-        else *(uint16_t *)dst = (uint16_t)w[0];
-        if (lane == 0) c.scales[row] = nan ? __uint_as_float(0x7fffffffu) : zero ? 0.f : __fdiv_rn(am, F);
+        kv8_load<E>((const T *)(kv ? a.v : a.k) + (int64_t)r * (kv ? a.v_row : a.k_row) + (int64_t)h * (kv ? a.v_head : a.k_head) + lane * E, x);
+        quantise_row<HD, FMT>(c, (size_t)kv8_row0(c, page, kv, h) + pos % KV8_PAGE, x);
     }
 }
 
-// The bounds of the blocks that got rows: the row with the newest position of its block does the block.  Bound: the latency of its rows.
-// grid (nb, kvh) x 256
-template <int HD, int FMT>
-__global__ void __launch_bounds__(256) kv8_bounds_k(Kv8Dev c, RowArgs a) {
-    constexpr uint32_t WC = HD / 4, NG = 256 / WC;  // columns of four channels, groups of tokens
+// A cache with bounds: the row with the newest position of its block stores all rows that the call has for the block, then goes over the block's keys for the
+// bounds; the other rows have nothing to do.  (Storing and bounds as two launches, with a search for the block's newest row in either: 5 + 9 us for 1024 rows of
+// the benchmark's layer, this MEASURE3.)  Bound: the latency of a block's rows.  grid (ceil(nb / per), kvh) x 512: a row per block of threads for up to 64 rows,
+// which mostly are of as many slots; four for more, which mostly are a prompt's (with one, 2000 blocks that find nothing to do took most of 14 us)
+template <int HD, int FMT, class T>
+__global__ void __launch_bounds__(512) kv8_put_blocks_k(Kv8Dev c, RowArgs a, uint32_t per) {
+    constexpr int E = HD / 32;
+    constexpr uint32_t WC = HD / 4, NG = 512 / WC;  // columns of four channels, groups of tokens
     __shared__ float lo_s[NG][HD], hi_s[NG][HD];
+    __shared__ int from[KV8_PAGE];  // of a token of the block: the last row for it, or -1
+    __shared__ uint32_t wm[16];
     pdl_sync();
-    const uint32_t r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, wc = tid % WC, tg = tid / WC;
-    const int slot = a.slots[r], pos = a.pos[r];
-    if (slot < 0 || pos < 0) return;
-    const int page = kv8_page(c, slot, pos / KV8_PAGE), blk = pos / (int)c.block;
-    if (page < 0) return;
-    bool newer = false;
-    for (uint32_t i = tid; i < a.nb; i += 256) {
-        const int p = a.pos[i];
-        newer |= a.slots[i] == slot && p >= 0 && p / (int)c.block == blk && (p > pos || (p == pos && i > r));
-    }
-    if (__syncthreads_or(newer)) return;
-    const uint32_t n = pos % c.block + 1;
-    const size_t row0 = (size_t)kv8_row0(c, page, 0, h) + blk * c.block % KV8_PAGE;
-    float lo[4], hi[4];
-    bool nan = false;
-#pragma unroll
-    for (int j = 0; j < 4; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
-#pragma unroll 4
-    for (uint32_t t = tg; t < n; t += NG) {
-        const uint32_t w = __ldcg((const uint32_t *)(c.codes + (row0 + t) * HD) + wc);
-        const float s = __ldcg(c.scales + row0 + t);
-        float x[4];
-        kv8_decode4<FMT>(w, x);
-        const bool bad = s != s;
-        nan |= bad;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float v = __fmul_rn(x[j], s);
-            if (!bad) lo[j] = fminf(lo[j], v), hi[j] = fmaxf(hi[j], v);
+    const uint32_t h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % WC, tg = tid / WC;
+    for (uint32_t r = blockIdx.x * per; r < a.nb && r < (blockIdx.x + 1) * per; r++) {  // (whether a row is passed over is the same for all threads)
+        const int slot = a.slots[r], pos = a.pos[r];
+        if (slot < 0 || pos < 0) continue;
+        const int blk = pos / (int)c.block;
+        auto newer = [&](uint32_t i) {  // row i makes row r one of the others (the same in all threads)
+            const int p = a.pos[i];
+            return a.slots[i] == slot && p >= 0 && p / (int)c.block == blk && (p > pos || (p == pos && i > r));
+        };
+        if ((r && newer(r - 1)) || (r + 1 < a.nb && newer(r + 1))) continue;  // (most rows of a prompt)
+        if (tid < c.block) from[tid] = -1;
+        __syncthreads();
+        bool other = false;
+        for (uint32_t i = tid; i < a.nb; i += 512) {
+            const int p = a.pos[i];
+            if (a.slots[i] != slot || p < 0 || p / (int)c.block != blk) continue;
+            other |= p > pos || (p == pos && i > r);
+            atomicMax(&from[p % c.block], (int)i);
         }
-    }
+        if (__syncthreads_or(other)) continue;
+        const int page = kv8_page(c, slot, pos / KV8_PAGE);
+        if (page < 0) {
+            if (tid == 0 && h == 0) set_status(c.status, ST_BAD_ARG | 0x21);
+            continue;
+        }
+        const uint32_t n = pos % c.block + 1;  // tokens of the block up to the newest
+        const size_t row0 = (size_t)kv8_row0(c, page, 0, h) + blk * c.block % KV8_PAGE, vrow0 = row0 + c.kvh * KV8_PAGE;
+        const T *kp = (const T *)a.k + (int64_t)h * a.k_head + lane * E, *vp = (const T *)a.v + (int64_t)h * a.v_head + lane * E;
+#pragma unroll 2
+        for (uint32_t p = warp; p < n; p += 16) {
+            const int i = from[p];
+            if (i < 0) continue;
+            float x[E], y[E];
+            kv8_load<E>(kp + (int64_t)i * a.k_row, x);
+            kv8_load<E>(vp + (int64_t)i * a.v_row, y);
+            quantise_row<HD, FMT>(c, row0 + p, x);
+            quantise_row<HD, FMT>(c, vrow0 + p, y);
+        }
+        __syncthreads();
+        // ---- bounds
+        float lo[4], hi[4];
+        bool nan = false;
 #pragma unroll
-    for (int j = 0; j < 4; j++) lo_s[tg][4 * wc + j] = lo[j], hi_s[tg][4 * wc + j] = hi[j];
-    nan = __syncthreads_or(nan);
-    float l = 0.f, u = 0.f;
-    if (tid < HD) {
-        l = lo_s[0][tid], u = hi_s[0][tid];
+        for (int j = 0; j < 4; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
+#pragma unroll 4
+        for (uint32_t t = tg; t < n; t += NG) {
+            const uint32_t w = __ldcg((const uint32_t *)(c.codes + (row0 + t) * HD) + wc);
+            const float s = __ldcg(c.scales + row0 + t);
+            float x[4];
+            kv8_decode4<FMT>(w, x);
+            const bool bad = s != s;
+            nan |= bad;
 #pragma unroll
-        for (uint32_t g = 1; g < NG; g++) l = fminf(l, lo_s[g][tid]), u = fmaxf(u, hi_s[g][tid]);
-        if (l > u) l = u = 0.f;  // every row is NaN
-    }
-    __shared__ uint32_t wm[8];
-    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(l), fabsf(u))));
-    if ((tid & 31) == 0) wm[tid >> 5] = m;
-    __syncthreads();
-    uint32_t b = 0;
+            for (int j = 0; j < 4; j++) {
+                const float v = __fmul_rn(x[j], s);
+                if (!bad) lo[j] = fminf(lo[j], v), hi[j] = fmaxf(hi[j], v);
+            }
+        }
 #pragma unroll
-    for (int i = 0; i < 8; i++) b = max(b, wm[i]);
-    const float bm = __uint_as_float(b);
-    const bool zero = bm < KV8_TINY;
-    const float inv = zero ? 0.f : __fdiv_rn(127.f, bm);
-    uint8_t *rec = c.bounds + kv8_bound_at(c, page, h, blk * c.block % KV8_PAGE / c.block);
-    if (tid < HD) {
-        rec[tid] = (uint8_t)(int8_t)fmaxf(-127.f, floorf(__fmul_rn(l, inv)));
-        rec[HD + tid] = (uint8_t)(int8_t)fminf(127.f, ceilf(__fmul_rn(u, inv)));
+        for (int j = 0; j < 4; j++) lo_s[tg][4 * wc + j] = lo[j], hi_s[tg][4 * wc + j] = hi[j];
+        nan = __syncthreads_or(nan);
+        float l = 0.f, u = 0.f;
+        if (tid < HD) {
+            l = lo_s[0][tid], u = hi_s[0][tid];
+#pragma unroll
+            for (uint32_t g = 1; g < NG; g++) l = fminf(l, lo_s[g][tid]), u = fmaxf(u, hi_s[g][tid]);
+            if (l > u) l = u = 0.f;  // every row is NaN
+        }
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(l), fabsf(u))));
+        if (lane == 0) wm[warp] = m;
+        __syncthreads();
+        uint32_t b = 0;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) b = max(b, wm[i]);
+        const float bm = __uint_as_float(b);
+        const bool zero = bm < KV8_TINY;
+        const float inv = zero ? 0.f : __fdiv_rn(127.f, bm);
+        uint8_t *rec = c.bounds + kv8_bound_at(c, page, h, blk * c.block % KV8_PAGE / c.block);
+        if (tid < HD) {
+            rec[tid] = (uint8_t)(int8_t)fmaxf(-127.f, floorf(__fmul_rn(l, inv)));
+            rec[HD + tid] = (uint8_t)(int8_t)fminf(127.f, ceilf(__fmul_rn(u, inv)));
+        }
+        if (tid < 4) ((float *)(rec + 2 * HD))[tid] = tid ? 0.f : nan ? INFINITY : zero ? 0.f : __fdiv_rn(bm, 127.f);
+        __syncthreads();
     }
-    if (tid < 4) ((float *)(rec + 2 * HD))[tid] = tid ? 0.f : nan ? INFINITY : zero ? 0.f : __fdiv_rn(bm, 127.f);
 }
 
 // ------------------------------------------------------------------------------------------------ rows out
@@ -175,10 +213,8 @@ typedef void (*row_kernel)(Kv8Dev, RowArgs);
                            : (dtype == QW_KV8_FP16 ? KV8_BY_DIM(NAME, QW_KV8_INT8, __half) : KV8_BY_DIM(NAME, QW_KV8_INT8, __nv_bfloat16)))
 row_kernel put_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_put_k); }
 row_kernel get_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_get_k); }
-row_kernel bounds_kernel(uint32_t hd, uint32_t format) {
-    if (format == QW_KV8_E4M3) return hd == 64 ? kv8_bounds_k<64, QW_KV8_E4M3> : hd == 128 ? kv8_bounds_k<128, QW_KV8_E4M3> : kv8_bounds_k<256, QW_KV8_E4M3>;
-    return hd == 64 ? kv8_bounds_k<64, QW_KV8_INT8> : hd == 128 ? kv8_bounds_k<128, QW_KV8_INT8> : kv8_bounds_k<256, QW_KV8_INT8>;
-}
+typedef void (*blocks_kernel)(Kv8Dev, RowArgs, uint32_t);
+blocks_kernel put_blocks_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_put_blocks_k); }
 
 const char *check_rows(const qw_kv8_cache *c, const qw_kv8_rows *a) {
     if (!a) return "no arguments";
@@ -190,9 +226,9 @@ RowArgs row_args(const qw_kv8_rows *a) { return {a->k, a->v, a->slots, a->pos, a
 
 cudaError_t enqueue_put(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_t st) {
     const Kv8Dev d = kv8_dev(c, a->layer);
-    cudaError_t e = qw_launch(put_kernel(c->hd, c->format, a->dtype), a->nb, 256, 0, st, d, row_args(a));
-    if (e == cudaSuccess && c->bounds) e = qw_launch(bounds_kernel(c->hd, c->format), dim3(a->nb, c->kvh), 256, 0, st, d, row_args(a));
-    return e;
+    const uint32_t per = a->nb <= 64 ? 1 : 4;
+    if (c->bounds) return qw_launch(put_blocks_kernel(c->hd, c->format, a->dtype), dim3((a->nb + per - 1) / per, c->kvh), 512, 0, st, d, row_args(a), per);
+    return qw_launch(put_kernel(c->hd, c->format, a->dtype), a->nb, 256, 0, st, d, row_args(a));
 }
 cudaError_t enqueue_get(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_t st) {
     return qw_launch(get_kernel(c->hd, c->format, a->dtype), a->nb, 256, 0, st, kv8_dev(c, a->layer), row_args(a));
@@ -225,7 +261,7 @@ cudaError_t rows_batch(const QwLaunch &L, enqueue_rows f) {
 cudaError_t launch_kv8_put(const QwLaunch &L) { return rows_batch(L, enqueue_put); }
 cudaError_t launch_kv8_get(const QwLaunch &L) { return rows_batch(L, enqueue_get); }
 }  // namespace
-QW_FAMILY(kv8_put, launch_kv8_put, 256)
+QW_FAMILY(kv8_put, launch_kv8_put, 512)
 QW_FAMILY(kv8_get, launch_kv8_get, 256)
 
 extern "C" int qw_kv8_put(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *err, size_t errlen) {

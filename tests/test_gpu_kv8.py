@@ -187,6 +187,29 @@ def test_the_later_of_two_rows_for_one_position_stays_and_unused_rows_are_passed
     assert int(rig.status) == 0
 
 
+@pytest.mark.parametrize("hd,kvh", [(64, 5), (128, 1), (256, 2)])
+def test_a_cache_without_bounds_stores_the_same_codes(hd, kvh):
+    rig = Rig([900, 70], kvh, hd, "int8", 64, layers=1, layer=0, seed=3)
+    plain = kv8.Kv8Cache(rig.t["codes"].clone(), rig.t["scales"].clone(), rig.t["table"], format="int8", status=rig.status)
+    s0, s1 = int(rig.slots[0]), int(rig.slots[1])
+    slots = np.array([s0] * 600 + [s1] * 3 + [-1, s0, s0])
+    pos = np.concatenate([np.arange(850, 250, -1), [0, 69, 0], [3, -1, 300]])  # (positions 0 and 300 twice)
+    n = len(slots)
+    k, v = rig.randn(n, kvh, hd, dtype=torch.bfloat16), rig.randn(n, kvh, hd, dtype=torch.bfloat16)
+    for c in (rig.cache, plain):
+        c.put(k, v, rig.idx(slots), rig.idx(pos))
+    for a, b in zip(rig.cache.tensors[:2], plain.tensors[:2]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    cc, ss = ref.quantise(host(k), "int8")
+    for r in (0, 599, 601, 602, n - 1):
+        assert np.array_equal(plain.tensors[0].cpu().numpy()[rig.table[slots[r], pos[r] // PAGE], 0, 0, :, pos[r] % PAGE], cc[r])
+    with pytest.raises(kv8.Kv8Error, match="bounds"):
+        plain.pick(rig.randn(2, kvh, hd), rig.idx(rig.lens), rig.idx(rig.slots), torch.zeros(2, kvh, 3, dtype=torch.int32, device="cuda"), max_len=900)
+    bad = rig.idx([99, s0])
+    plain.put(k[:2].contiguous(), v[:2].contiguous(), bad, rig.idx([0, 10 ** 6]))
+    assert int(rig.status) & 0xf00 == 0x200
+
+
 def test_rows_outside_the_cache_are_dropped_and_reported():
     rig = Rig([300], 2, 128, "int8", 64, layers=1, layer=0)
     n_slots = rig.table.shape[0]
