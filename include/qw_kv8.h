@@ -5,8 +5,8 @@
  * Pages hold 256 tokens, as the fp16 cache's do.  A row is one token's key or value of one kv head:
  *   a = max |x|;  scale = a / F;  code = nearest(x * (F / a))      F = 448 (e4m3) or 127 (int8), every operation rounded to fp32
  * and code * scale is what the row stands for.  A row whose a is below 2^-100 is stored as zeros with scale 0; one that holds an infinity or a NaN
- * gets scale NaN, so that whatever attends to it turns NaN.  An e4m3 cache holds no NaN codes; where a host writes codes itself, 0x7f and 0xff
- * stand for 480 and -480 times the scale, not for NaN.
+ * gets scale NaN, so that whatever attends to it turns NaN.  A host that writes codes itself does not use the e4m3 codes 0x7f and 0xff, nor infinite or
+ * negative scales, in rows that are looked at; rows behind a slot's last token may hold anything.
  *
  * All pointers are device pointers of the device that is current and that `stream` (a cudaStream_t) belongs to; buffers of another device are
  * refused.  Calls only enqueue work: they do not allocate, do not wait and may be captured into a CUDA graph.  Calls that share a workspace
@@ -45,7 +45,7 @@ typedef struct {
 int qw_kv8_bytes(const qw_kv8_cache *c, size_t out[3]);
 
 /* Row r (of nb <= 1024) goes to / comes from position pos[r] of slot slots[r]; rows with a negative slot or position are skipped (get: the output row
- * stays as it was).  k and v: [nb][kvh][hd] with these strides in elements; a row's hd values are contiguous. */
+ * stays as it was).  k and v: [nb][kvh][hd] with these strides in elements, of any alignment; a row's hd values are contiguous. */
 typedef struct {
     void *k, *v;
     const int32_t *slots, *pos; /* [nb] */
@@ -64,7 +64,8 @@ int qw_kv8_get(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *
 
 /* Attention of one new token per row over its slot's first lens[r] tokens: y = sum_t softmax_t(scale * q . k_t) v_t for each of the qh query heads
  * (qh / kvh = 1 .. 16 of them share a kv head, as consecutive ones), times sigmoid(gate) where there is a gate.  A row of length 0 is zero; a row with
- * a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks], distinct block numbers, negative = none) the tokens are those of the named blocks.
+ * a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks], distinct block numbers, the first
+ * negative one ends them) the tokens are those of the named blocks.  An infinity or a NaN in a query makes its head's result NaN.
  * max_len: no row is longer (a longer one is answered with NaN).  What a row yields does not depend on the other rows of the call.
  * work: qw_kv8_attn_work(...) bytes, 16-byte aligned, nothing has to be in it. */
 typedef struct {

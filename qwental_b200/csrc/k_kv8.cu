@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
 
 // A cache with bounds: the row with the newest position of its block stores all rows that the call has for the block, then goes over the block's keys for the
 // bounds; the other rows have nothing to do.  (Storing and bounds as two launches, with a search for the block's newest row in either: 5 + 9 us for 1024 rows of
-// the benchmark's layer, this MEASURE3.)  Bound: the latency of a block's rows.  grid (ceil(nb / per), kvh) x 512: a row per block of threads for up to 64 rows,
+// the benchmark's layer, this 9.)  Bound: the latency of a block's rows.  grid (ceil(nb / per), kvh) x 512: a row per block of threads for up to 64 rows,
 // which mostly are of as many slots; four for more, which mostly are a prompt's (with one, 2000 blocks that find nothing to do took most of 14 us)
 template <int HD, int FMT, class T>
 __global__ void __launch_bounds__(512) kv8_put_blocks_k(Kv8Dev c, RowArgs a, uint32_t per) {
@@ -234,10 +234,15 @@ cudaError_t enqueue_get(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_
     return qw_launch(get_kernel(c->hd, c->format, a->dtype), a->nb, 256, 0, st, kv8_dev(c, a->layer), row_args(a));
 }
 
+const char *check_out(const qw_kv8_cache *c, const qw_kv8_rows *a) {
+    if ((a->nb > 1 && (!a->k_row || !a->v_row)) || (c->kvh > 1 && (!a->k_head || !a->v_head))) return "results that lie on one another";
+    return nullptr;
+}
 typedef cudaError_t (*enqueue_rows)(const qw_kv8_cache *, const qw_kv8_rows *, cudaStream_t);
 int rows_call(const char *where, enqueue_rows f, const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *err, size_t errlen) {
     const char *m = kv8_check_cache(c);
     if (!m) m = check_rows(c, a);
+    if (!m && f == enqueue_get) m = check_out(c, a);
     if (m) return kv8_fail(-1, where, m, err, errlen);
     const void *ptrs[] = {c->codes, c->scales, c->bounds, c->page_table, c->status, a->k, a->v, a->slots, a->pos};
     if ((m = kv8_check_device(ptrs, 9))) return kv8_fail(-3, where, m, err, errlen);
@@ -254,7 +259,7 @@ cudaError_t rows_batch(const QwLaunch &L, enqueue_rows f) {
     QW_CHECK_ARG(kv8_from_binds(L, &c, &s) && L.has_bytes(8, 32));
     struct { int64_t s[4]; } st = L.bytes<decltype(st)>(8);
     const qw_kv8_rows a = {L.buf<void>(4), L.buf<void>(5), L.buf<int32_t>(6), L.buf<int32_t>(7), st.s[0], st.s[1], st.s[2], st.s[3], s.nb, s.layer, s.dtype, 0};
-    QW_CHECK_ARG(!check_rows(&c, &a) && L.avail(6) >= (size_t)s.nb * 4 && L.avail(7) >= (size_t)s.nb * 4);
+    QW_CHECK_ARG(!check_rows(&c, &a) && (f != enqueue_get || !check_out(&c, &a)) && L.avail(6) >= (size_t)s.nb * 4 && L.avail(7) >= (size_t)s.nb * 4);
     QW_CHECK_ARG(kv8_rows_fit(L, 4, s.nb, s.kvh, s.hd, a.k_row, a.k_head) && kv8_rows_fit(L, 5, s.nb, s.kvh, s.hd, a.v_row, a.v_head));
     return f(&c, &a, L.stream);
 }

@@ -12,7 +12,7 @@ using namespace qw;
 
 namespace {
 // Tokens of a chunk, by the tokens of its row alone (a row's result does not depend on the others of a call): short rows in small pieces, for their latency;
-// a chunk of 128 leaves 12 % of its own bytes as fp32 sums, in L2.  With 256 from 8193 tokens on, one row of 48000 took 24 us instead of MEASURE1 and 16 ragged rows
+// a chunk of 128 leaves 12 % of its own bytes as fp32 sums, in L2.  With 256 from 8193 tokens on, one row of 48000 took 24 us instead of 20 and 16 ragged rows
 // of 1K to 48K had single warps that ended 9 us after the others.
 __host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 65536 ? 7 : 8; }
 __host__ __device__ inline uint32_t chunk_of(uint32_t n) { return 1u << chunk_log(n); }
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 const __half2 h2 = __floats2half2_rn(f.x * down, f.y * down);
                 qf[nt][x] = head < a.G ? *(const uint32_t *)&h2 : 0u;
             }
-            const float f = up * a.scale2;
+            const float f = m >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : up * a.scale2;  // an infinity or a NaN: the head's results are NaN
             fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
             fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
         }
@@ -679,6 +679,7 @@ int check_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, const char **m)
     if ((*m = kv8_check_layer(c, a->nb, a->layer, a->dtype)) || (*m = check_shape(c, a->nb, a->qh, a->max_len))) return -1;
     if (!a->q || !a->y || !a->lens || !a->slots || !a->work) return *m = "null pointer argument", -1;
     if (a->blocks && a->nblocks < 1) return *m = "chosen blocks of no number", -1;
+    if ((a->nb > 1 && !a->y_row) || (a->qh > 1 && !a->y_head)) return *m = "results that lie on one another", -1;
     if ((uintptr_t)a->work & 15) return *m = "the workspace starts at a 16-byte boundary", -1;
     if (!(a->scale > 0.f) || a->scale > 1e30f) return *m = "the softmax scale is a positive number", -1;
     if (a->work_bytes < work_of(c, a->nb, a->qh, a->max_len, a->blocks ? a->nblocks : 0)) return *m = "the workspace is too small", -2;

@@ -1,6 +1,7 @@
 """Python face of the 8-bit key-value cache (include/qw_kv8.h) for hosts that hold their memory as torch tensors: rows in and out,
 attention of one new token per row, and the choice of blocks.  All work happens in libqw_gpu_cuda.so, on torch's current stream (or the
-one that is given); nothing waits, and every call may be captured into a CUDA graph.  Errors raise Kv8Error with the library's message.
+one that is given, as a cudaStream_t); nothing waits, and every call may be captured into a CUDA graph.  Tensors have to outlive the work on them: one that was made on
+another stream than the call's is the caller's to record there.  Errors raise Kv8Error with the library's message.
 """
 from __future__ import annotations
 
@@ -123,8 +124,10 @@ class Kv8Cache:
             raise Kv8Error("blocks are int32 [%d, %d, n] on the cache's device" % (nb, self.kvh))
         return t.data_ptr(), t.shape[2]
 
-    def _work(self, work, need):
+    def _work(self, work, need, stream):
         if work is None:
+            if stream is not None:  # it would go back to torch's allocator while that stream still uses it
+                raise Kv8Error("a call on a stream that is given needs a workspace that is given")
             work = torch.empty(max(16, need), dtype=torch.uint8, device=self.device)
         if work.get_device() != self.index or not work.is_contiguous():
             raise Kv8Error("the workspace is contiguous and on the cache's device")
@@ -179,7 +182,7 @@ class Kv8Cache:
         yp, yr, yd = self._rows(y, nb, qh, q.dtype, "y")
         gp, gr, gd = (None, 0, 0) if gate is None else self._rows(gate, nb, qh, q.dtype, "gate")
         bp, nblocks = (None, 0) if blocks is None else self._blocks(blocks, nb)
-        work, wp, size = self._work(work, self.L.qw_kv8_attn_work(self._ref, nb, qh, max_len, nblocks) if work is None else 0)
+        work, wp, size = self._work(work, self.L.qw_kv8_attn_work(self._ref, nb, qh, max_len, nblocks) if work is None else 0, stream)
         self._call(self.L.qw_kv8_attn, AttnStruct(qp, gp, yp, self._index(lens, nb, "lens"), self._index(slots, nb, "slots"), bp, wp, size, qr, qd, gr, gd, yr, yd,
                                                   self.hd ** -0.5 if scale is None else scale, nb, layer, dt, qh, max_len, nblocks), stream)
         return y
@@ -189,7 +192,7 @@ class Kv8Cache:
         nb, qh, dt = lens.shape[0], q.shape[1] if q.dim() == 3 else 0, self._dtype(q, "q")
         qp, qr, qd = self._rows(q, nb, qh, q.dtype, "q")
         bp, nblocks = self._blocks(blocks, nb)
-        work, wp, size = self._work(work, self.L.qw_kv8_pick_work(self._ref, nb, max_len) if work is None else 0)
+        work, wp, size = self._work(work, self.L.qw_kv8_pick_work(self._ref, nb, max_len) if work is None else 0, stream)
         self._call(self.L.qw_kv8_pick, PickStruct(qp, self._index(lens, nb, "lens"), self._index(slots, nb, "slots"), bp, wp, size, qr, qd, nb, layer, dt, qh, max_len, nblocks,
                                                   first, last), stream)
         return blocks

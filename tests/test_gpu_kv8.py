@@ -313,6 +313,21 @@ def test_attention_at_the_ends_of_the_ranges(qs, vs, ks, fmt):
     check_attention(rig, q, y, torch.bfloat16, scale=sc)
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_query_that_holds_no_numbers_spoils_its_head_alone(bad):
+    rig = Rig([300, 1], 2, 128, "e4m3", layers=1, layer=0, seed=12)
+    rig.codes[:, :, 0] &= 0x7f  # keys of one sign: a query of -infinity has no score but -infinity
+    rig.t["codes"].copy_(torch.from_numpy(rig.codes))
+    q = rig.randn(2, 12, 128)
+    q[0, 7, 5] = bad
+    q[1, 0, 127] = bad
+    y = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=300)
+    gone = torch.zeros(2, 12, dtype=torch.bool)
+    gone[0, 7] = gone[1, 0] = True
+    assert torch.equal(y.isnan().all(-1).cpu(), gone) and torch.equal(y.isnan().any(-1).cpu(), gone)
+
+
 def test_a_single_token_that_wins_everything():
     """Scores far apart: the row is that token's value."""
     rig = Rig([500, 500], 1, 64, "int8", layers=1, layer=0, seed=9)
@@ -581,6 +596,8 @@ def test_streams_and_captured_graphs():
     work = [torch.empty(rig.cache.work_bytes(n, 16, 1500), dtype=torch.uint8, device="cuda") for _ in range(2)]
     got = [(torch.zeros_like(q[i]), torch.zeros_like(want[i][1])) for i in range(2)]
     torch.cuda.synchronize()
+    with pytest.raises(kv8.Kv8Error, match="workspace"):
+        rig.cache.attn(q[0], lens[0], slots, got[0][0], layer=L, max_len=1500, stream=streams[0].cuda_stream)
     for _ in range(20):
         for i in range(2):
             rig.cache.pick(q[i], lens[i], slots, got[i][1], layer=L, max_len=1500, work=work[i], stream=streams[i].cuda_stream)

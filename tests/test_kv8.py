@@ -64,11 +64,20 @@ def test_bad_rows_are_refused(name, over, msg):
     assert rc == -1 and msg in m
 
 
+@pytest.mark.parametrize("over", [dict(k_row=0), dict(v_row=0), dict(k_head=0), dict(v_head=0)])
+def test_rows_read_back_onto_one_another_are_refused(over):
+    rc, m = call("qw_kv8_get", cache(), rows(**over))
+    assert rc == -1 and "on one another" in m
+    rc, m = call("qw_kv8_put", cache(), rows(**over))  # one row for many places is fine
+    assert rc != -1
+
+
 @pytest.mark.parametrize("over,code,msg", [(dict(nb=0), -1, "1 to 1024"), (dict(layer=2), -1, "layer"), (dict(dtype=7), -1, "type"), (dict(qh=0), -1, "query heads"), (dict(qh=7), -1, "query heads"),
                                            (dict(qh=51), -1, "query heads"), (dict(max_len=0), -1, "max_len"), (dict(max_len=6 * 256 + 1), -1, "max_len"), (dict(q=None), -1, "null"),
                                            (dict(y=None), -1, "null"), (dict(lens=None), -1, "null"), (dict(slots=None), -1, "null"), (dict(work=None), -1, "null"),
                                            (dict(work=4104), -1, "16-byte"), (dict(blocks=4096), -1, "no number"), (dict(scale=0.0), -1, "scale"), (dict(scale=-1.0), -1, "scale"),
-                                           (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(work_bytes=16), -2, "too small")])
+                                           (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(y_row=0), -1, "on one another"),
+                                           (dict(y_head=0), -1, "on one another"), (dict(work_bytes=16), -2, "too small")])
 def test_bad_attention_is_refused(over, code, msg):
     rc, m = call("qw_kv8_attn", cache(), attn(**over))
     assert rc == code and msg in m
@@ -80,6 +89,12 @@ def test_bad_attention_is_refused(over, code, msg):
 def test_a_bad_choice_is_refused(over, code, msg):
     rc, m = call("qw_kv8_pick", cache(), pick(**over))
     assert rc == code and msg in m
+
+
+def test_more_tokens_than_a_call_takes_are_refused():
+    big = dict(pages=1000, max_pages=1 << 22, kvh=64, layers=1, hd=64)
+    rc, m = call("qw_kv8_attn", cache(**big), attn(layer=0, qh=64, nb=1024, max_len=(1 << 30) - 1, q_head=64, y_head=64))
+    assert rc == -1 and "more tokens" in m
 
 
 def test_a_choice_needs_bounds():
