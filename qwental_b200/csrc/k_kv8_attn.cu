@@ -698,7 +698,8 @@ cudaError_t enqueue_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, cudaS
     const uint64_t most = (uint64_t)a->nb * mc * c->kvh, sms = (uint64_t)kv8_sm_count();
     const Launch L = launch_of(c->hd, c->format, a->dtype, k.G, most <= 6 * sms);
     const int smem = L.smem + (int)a->nb * 12;
-    cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // (the most of any call: another thread's call, or a captured one, may be of more rows than this)
+    cudaError_t e = cudaFuncSetAttribute(L.core, cudaFuncAttributeMaxDynamicSharedMemorySize, L.smem + 12 * KV8_MAX_ROWS);
     if (e != cudaSuccess) return e;
     e = qw_launch(L.core, (uint32_t)(most < sms ? most : sms), L.threads, smem, st, tm, d, k, box_rows, status);
     if (e != cudaSuccess) return e;

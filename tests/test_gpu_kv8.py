@@ -629,6 +629,45 @@ def test_streams_and_captured_graphs():
             assert torch.equal(got[i][0], want[i ^ swap][0]) and torch.equal(got[i][1], want[i ^ swap][1])
 
 
+def test_calls_of_few_and_of_many_rows_from_two_threads():
+    """What a call needs of a kernel that another call uses too (its shared memory grows with the rows) does not depend on who comes last; the same for a
+    captured call of many rows, replayed after a call of few."""
+    import threading
+    rig = Rig([300] * 64, 1, 64, "int8", seed=7)
+    big = np.tile(np.arange(64), 16)
+    lens, slots = rig.idx(rig.lens[big]), rig.idx(rig.slots[big])
+    q = rig.randn(1024, 4, 64)
+    want = torch.zeros_like(q)
+    rig.cache.attn(q, lens, slots, want, layer=1, max_len=512)
+    counts = (1024, 200)  # both of more tasks than the variant for few takes
+    got = [torch.zeros_like(q) for _ in counts]
+    work = [torch.empty(rig.cache.work_bytes(1024, 4, 512), dtype=torch.uint8, device="cuda") for _ in counts]
+    streams = [torch.cuda.Stream() for _ in counts]
+    graph, y = torch.cuda.CUDAGraph(), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        rig.cache.attn(q, lens, slots, y, layer=1, max_len=512)
+    errors = []
+
+    def run(i):
+        try:
+            n = counts[i]
+            c = kv8.Kv8Cache(rig.t["codes"], rig.t["scales"], rig.t["table"], rig.t["bounds"], format="int8")
+            for _ in range(200):
+                c.attn(q[:n], lens[:n], slots[:n], got[i][:n], layer=1, max_len=512, work=work[i], stream=streams[i].cuda_stream)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for g, n in list(zip(got, counts)) + [(y, 1024)]:
+        assert torch.equal(g[:n], want[:n])
+
+
 def test_buffers_of_other_places_are_refused():
     rig = Rig([100], 1, 64, "int8", layers=1, layer=0)
     a = kv8.RowsStruct()
