@@ -220,6 +220,8 @@ const char *check_rows(const qw_kv8_cache *c, const qw_kv8_rows *a) {
     if (!a) return "no arguments";
     if (const char *m = kv8_check_layer(c, a->nb, a->layer, a->dtype)) return m;
     if (!a->k || !a->v || !a->slots || !a->pos) return "null pointer argument";
+    const void *ptrs[] = {a->k, a->v, a->slots, a->pos};
+    if (!kv8_aligned(2, 2, ptrs)) return "a tensor does not start at a boundary of its type";
     return nullptr;
 }
 RowArgs row_args(const qw_kv8_rows *a) { return {a->k, a->v, a->slots, a->pos, a->k_row, a->k_head, a->v_row, a->v_head, a->nb}; }
@@ -235,7 +237,7 @@ cudaError_t enqueue_get(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_
 }
 
 const char *check_out(const qw_kv8_cache *c, const qw_kv8_rows *a) {
-    if ((a->nb > 1 && (!a->k_row || !a->v_row)) || (c->kvh > 1 && (!a->k_head || !a->v_head))) return "results that lie on one another";
+    if (kv8_overlap(a->nb, c->kvh, c->hd, a->k_row, a->k_head) || kv8_overlap(a->nb, c->kvh, c->hd, a->v_row, a->v_head)) return "results that lie on one another";
     return nullptr;
 }
 typedef cudaError_t (*enqueue_rows)(const qw_kv8_cache *, const qw_kv8_rows *, cudaStream_t);
@@ -292,6 +294,7 @@ const char *kv8_check_cache(const qw_kv8_cache *c) {
     if (const char *m = check_sizes(c)) return m;
     if (!c->codes || !c->scales || !c->page_table) return "null pointer in the cache";
     if (((uintptr_t)c->codes | (uintptr_t)c->scales | (uintptr_t)c->bounds) & 15) return "codes, scales and bounds start at 16-byte boundaries";
+    if (((uintptr_t)c->page_table | (uintptr_t)c->status) & 3) return "page table and status start at 4-byte boundaries";
     return nullptr;
 }
 const char *kv8_check_layer(const qw_kv8_cache *c, uint32_t nb, uint32_t layer, uint32_t dtype) {
@@ -302,6 +305,11 @@ const char *kv8_check_layer(const qw_kv8_cache *c, uint32_t nb, uint32_t layer, 
 }
 Kv8Dev kv8_dev(const qw_kv8_cache *c, uint32_t layer) {
     return {c->codes, c->scales, c->bounds, c->page_table, c->status, c->pages, c->layers, c->kvh, c->hd, c->block, c->slots, c->max_pages, layer};
+}
+bool kv8_aligned(int n2, int n4, const void *const *ptrs) {
+    for (int i = 0; i < n2 + n4; i++)
+        if ((uintptr_t)ptrs[i] & (i < n2 ? 1 : 3)) return false;
+    return true;
 }
 int kv8_fail(int code, const char *where, const char *msg, char *err, size_t errlen) {
     if (err && errlen) snprintf(err, errlen, "qw_%s: %s", where, msg);

@@ -91,6 +91,30 @@ def test_a_bad_choice_is_refused(over, code, msg):
     assert rc == code and msg in m
 
 
+@pytest.mark.parametrize("name,args,fields", [("qw_kv8_put", rows, "k v slots pos"), ("qw_kv8_get", rows, "k v slots pos"), ("qw_kv8_attn", attn, "q y gate lens slots"),
+                                              ("qw_kv8_pick", pick, "q lens slots blocks")])
+def test_pointers_between_elements_are_refused(name, args, fields):
+    for f in fields.split():
+        for off in (1, 2) if f in ("slots", "pos", "lens", "blocks") else (1,):
+            rc, m = call(name, cache(), args(**{f: 4096 + off}))
+            assert rc == -1 and "boundary" in m, f
+    rc, m = call("qw_kv8_attn", cache(), attn(blocks=4098, nblocks=2))
+    assert rc == -1 and "boundary" in m
+    for over in (dict(page_table=4098), dict(status=4097)):
+        rc, m = call(name, cache(**over), args())
+        assert rc == -1 and "4-byte" in m
+
+
+def test_results_closer_than_a_row_is_long_are_refused():
+    for name, args, fields in (("qw_kv8_get", rows, "k_row k_head v_row v_head"), ("qw_kv8_attn", attn, "y_row y_head")):
+        for f in fields.split():
+            for x in (127, -127, 1):
+                rc, m = call(name, cache(), args(**{f: x}))
+                assert rc == -1 and "on one another" in m
+    for name, args, over in (("qw_kv8_put", rows, dict(k_row=1, k_head=3)), ("qw_kv8_attn", attn, dict(q_row=1, gate_head=0)), ("qw_kv8_pick", pick, dict(q_head=1))):
+        assert "on one another" not in call(name, cache(), args(**over))[1]  # what is read may overlap
+
+
 def test_more_tokens_than_a_call_takes_are_refused():
     big = dict(pages=1000, max_pages=1 << 22, kvh=64, layers=1, hd=64)
     rc, m = call("qw_kv8_attn", cache(**big), attn(layer=0, qh=64, nb=1024, max_len=(1 << 30) - 1, q_head=64, y_head=64))
