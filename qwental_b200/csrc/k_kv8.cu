@@ -66,57 +66,96 @@ __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
     }
 }
 
-// A cache with bounds: the row with the newest position of its block stores all rows that the call has for the block, then goes over the block's keys for the
-// bounds; the other rows have nothing to do.  (Storing and bounds as two launches, with a search for the block's newest row in either: 5 + 9 us for 1024 rows of
-// the benchmark's layer, this 9.)  Bound: the latency of a block's rows.  grid (ceil(nb / per), kvh) x 512: a row per block of threads for up to 64 rows,
-// which mostly are of as many slots; four for more, which mostly are a prompt's (with one, 2000 blocks that find nothing to do took most of 14 us)
+// A cache with bounds: of the rows for one block (16 to 256 tokens) the one with the newest position, its leader, stores all of them and then goes over the
+// block's keys for the bounds.  The call's slots and positions are put into shared memory first; a row is asked after if neither of its neighbours in the call is of the same
+// block and newer (most rows of a prompt are not), and leads if no other row is.  Keys (with the bounds) and values are different blocks of threads.
+// Bound: the latency of one after the other: rows' numbers, their values, the block's keys from L2.  From a captured graph, per call: 16 rows (hd 256, 2 kv heads) 5.4 us, 419
+// (hd 128, 8 kv heads) 7.1, 1024 (hd 256, 2 kv heads) 8.9; with the search in global memory and keys and values in the same block 5.3, 14.5 and 14.3; with that list of
+// rows for calls of a row per block of threads too, 6.2 for the 16.
+// grid (blocks of threads that share the leaders, 2 kvh) x 512
 template <int HD, int FMT, class T>
-__global__ void __launch_bounds__(512) kv8_put_blocks_k(Kv8Dev c, RowArgs a, uint32_t per) {
+__global__ void __launch_bounds__(512, 2) kv8_put_blocks_k(Kv8Dev c, RowArgs a) {
     constexpr int E = HD / 32;
     constexpr uint32_t WC = HD / 4, NG = 512 / WC;  // columns of four channels, groups of tokens
+    static_assert(KV8_MAX_ROWS == 1024, "two rows per thread");
     __shared__ float lo_s[NG][HD], hi_s[NG][HD];
+    __shared__ int slot_s[KV8_MAX_ROWS], pos_s[KV8_MAX_ROWS];
+    __shared__ uint16_t asked[KV8_MAX_ROWS];
     __shared__ int from[KV8_PAGE];  // of a token of the block: the last row for it, or -1
-    __shared__ uint32_t wm[16];
+    __shared__ uint32_t wm[32];
     pdl_sync();
-    const uint32_t h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % WC, tg = tid / WC;
-    for (uint32_t r = blockIdx.x * per; r < a.nb && r < (blockIdx.x + 1) * per; r++) {  // (whether a row is passed over is the same for all threads)
-        const int slot = a.slots[r], pos = a.pos[r];
-        if (slot < 0 || pos < 0) continue;
-        const int blk = pos / (int)c.block;
-        auto newer = [&](uint32_t i) {  // row i makes row r one of the others (the same in all threads)
-            const int p = a.pos[i];
-            return a.slots[i] == slot && p >= 0 && p / (int)c.block == blk && (p > pos || (p == pos && i > r));
-        };
-        if ((r && newer(r - 1)) || (r + 1 < a.nb && newer(r + 1))) continue;  // (most rows of a prompt)
+    const uint32_t kv = blockIdx.y >= c.kvh, h = blockIdx.y - kv * c.kvh, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wc = tid % WC, tg = tid / WC;
+    const int bl = 31 - __clz(c.block);  // (a power of two)
+    int sl[2], ps[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const uint32_t i = e * 512 + tid;
+        sl[e] = i < a.nb ? a.slots[i] : -1;
+        ps[e] = i < a.nb ? a.pos[i] : -1;
+        slot_s[i] = sl[e], pos_s[i] = ps[e];
+    }
+    __syncthreads();
+    auto newer = [&](uint32_t i, uint32_t r) {  // row i is of row r's block and newer (row r is in use)
+        const int p = pos_s[i], q = pos_s[r];
+        return slot_s[i] == slot_s[r] && p >= 0 && p >> bl == q >> bl && (p > q || (p == q && i > r));
+    };
+    uint32_t all = a.nb;
+    const bool each = gridDim.x == a.nb;  // a row for every block of threads: no list of the rows to ask after
+    if (!each) {
+        uint32_t ask[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t i = e * 512 + tid;
+            ask[e] = __ballot_sync(0xffffffffu, sl[e] >= 0 && ps[e] >= 0 && !(i && newer(i - 1, i)) && !(i + 1 < a.nb && newer(i + 1, i)));
+            if (lane == 0) wm[e * 16 + warp] = __popc(ask[e]);
+        }
+        __syncthreads();
+        const uint32_t in_warps = wm[lane];
+        all = __reduce_add_sync(0xffffffffu, in_warps);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t at = __reduce_add_sync(0xffffffffu, lane < e * 16 + warp ? in_warps : 0u);
+            if (ask[e] >> lane & 1) asked[at + __popc(ask[e] & ((1u << lane) - 1))] = (uint16_t)(e * 512 + tid);
+        }
+    }
+    for (uint32_t z = blockIdx.x; z < all; z += gridDim.x) {
         if (tid < c.block) from[tid] = -1;
         __syncthreads();
+        const uint32_t r = each ? z : asked[z];
+        const int slot = slot_s[r], pos = pos_s[r], blk = pos >> bl;
+        if (slot < 0 || pos < 0) continue;
+        const int page = kv8_page(c, slot, pos / KV8_PAGE);
         bool other = false;
-        for (uint32_t i = tid; i < a.nb; i += 512) {
-            const int p = a.pos[i];
-            if (a.slots[i] != slot || p < 0 || p / (int)c.block != blk) continue;
-            other |= p > pos || (p == pos && i > r);
-            atomicMax(&from[p % c.block], (int)i);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t i = e * 512 + tid;
+            if (sl[e] != slot || ps[e] < 0 || ps[e] >> bl != blk) continue;
+            other |= ps[e] > pos || (ps[e] == pos && i > r);
+            atomicMax(&from[ps[e] & (c.block - 1)], (int)i);
         }
         if (__syncthreads_or(other)) continue;
-        const int page = kv8_page(c, slot, pos / KV8_PAGE);
         if (page < 0) {
-            if (tid == 0 && h == 0) set_status(c.status, ST_BAD_ARG | 0x21);
+            if (tid == 0 && blockIdx.y == 0) set_status(c.status, ST_BAD_ARG | 0x21);
             continue;
         }
         const uint32_t n = pos % c.block + 1;  // tokens of the block up to the newest
-        const size_t row0 = (size_t)kv8_row0(c, page, 0, h) + blk * c.block % KV8_PAGE, vrow0 = row0 + c.kvh * KV8_PAGE;
-        const T *kp = (const T *)a.k + (int64_t)h * a.k_head + lane * E, *vp = (const T *)a.v + (int64_t)h * a.v_head + lane * E;
-#pragma unroll 2
-        for (uint32_t p = warp; p < n; p += 16) {
-            const int i = from[p];
-            if (i < 0) continue;
-            float x[E], y[E];
-            kv8_load<E>(kp + (int64_t)i * a.k_row, x);
-            kv8_load<E>(vp + (int64_t)i * a.v_row, y);
-            quantise_row<HD, FMT>(c, row0 + p, x);
-            quantise_row<HD, FMT>(c, vrow0 + p, y);
+        const size_t row0 = (size_t)kv8_row0(c, page, kv, h) + blk * c.block % KV8_PAGE;
+        const T *src = kv ? (const T *)a.v + (int64_t)h * a.v_head + lane * E : (const T *)a.k + (int64_t)h * a.k_head + lane * E;
+        const int64_t stride = kv ? a.v_row : a.k_row;
+        for (uint32_t p0 = warp; p0 < n; p0 += 64) {  // four rows at a time, all loads before the first store
+            float x[4][E];
+            int i[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                i[j] = p0 + 16 * j < n ? from[p0 + 16 * j] : -1;
+                if (i[j] >= 0) kv8_load<E>(src + (int64_t)i[j] * stride, x[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i[j] >= 0) quantise_row<HD, FMT>(c, row0 + p0 + 16 * j, x[j]);
         }
         __syncthreads();
+        if (kv) continue;
         // ---- bounds
         float lo[4], hi[4];
         bool nan = false;
@@ -213,8 +252,7 @@ typedef void (*row_kernel)(Kv8Dev, RowArgs);
                            : (dtype == QW_KV8_FP16 ? KV8_BY_DIM(NAME, QW_KV8_INT8, __half) : KV8_BY_DIM(NAME, QW_KV8_INT8, __nv_bfloat16)))
 row_kernel put_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_put_k); }
 row_kernel get_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_get_k); }
-typedef void (*blocks_kernel)(Kv8Dev, RowArgs, uint32_t);
-blocks_kernel put_blocks_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_put_blocks_k); }
+row_kernel put_blocks_kernel(uint32_t hd, uint32_t format, uint32_t dtype) { return KV8_BY_ALL(kv8_put_blocks_k); }
 
 const char *check_rows(const qw_kv8_cache *c, const qw_kv8_rows *a) {
     if (!a) return "no arguments";
@@ -228,8 +266,10 @@ RowArgs row_args(const qw_kv8_rows *a) { return {a->k, a->v, a->slots, a->pos, a
 
 cudaError_t enqueue_put(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_t st) {
     const Kv8Dev d = kv8_dev(c, a->layer);
-    const uint32_t per = a->nb <= 64 ? 1 : 4;
-    if (c->bounds) return qw_launch(put_blocks_kernel(c->hd, c->format, a->dtype), dim3((a->nb + per - 1) / per, c->kvh), 512, 0, st, d, row_args(a), per);
+    if (c->bounds) {  // about as many blocks of threads as are resident at once, or fewer
+        const uint32_t most = c->kvh < 256 ? 256 / c->kvh : 1;
+        return qw_launch(put_blocks_kernel(c->hd, c->format, a->dtype), dim3(a->nb < most ? a->nb : most, 2 * c->kvh), 512, 0, st, d, row_args(a));
+    }
     return qw_launch(put_kernel(c->hd, c->format, a->dtype), a->nb, 256, 0, st, d, row_args(a));
 }
 cudaError_t enqueue_get(const qw_kv8_cache *c, const qw_kv8_rows *a, cudaStream_t st) {
@@ -285,7 +325,7 @@ static const char *check_sizes(const qw_kv8_cache *c) {
     if (c->format != QW_KV8_E4M3 && c->format != QW_KV8_INT8) return "unknown format";
     if (c->block < 16 || c->block > KV8_PAGE || (c->block & (c->block - 1))) return "a block has 16, 32, 64, 128 or 256 tokens";
     if (c->pages < 1 || c->layers < 1 || c->kvh < 1 || c->slots < 1 || c->max_pages < 1) return "a cache has at least one page, layer, kv head, slot and page per slot";
-    if (c->kvh > 65535) return "too many kv heads";
+    if (c->kvh > 32767) return "too many kv heads";
     if ((double)c->pages * c->layers * 2 * c->kvh * KV8_PAGE > 2147483647.0) return "more than 2^31 - 1 rows";
     if (c->max_pages > 0x7fffffffu / KV8_PAGE || c->slots > 0x7fffffffu) return "a slot has at most 2^31 - 1 tokens";
     return nullptr;
