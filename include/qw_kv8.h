@@ -53,7 +53,8 @@ typedef struct {
     uint32_t nb, layer, dtype, reserved;
 } qw_kv8_rows;
 
-/* Quantises the rows into the cache.  Of two rows for the same position the later one stays.  Where the cache has bounds, those of every block that
+/* Quantises the rows into the cache.  Of two rows for the same position the later one stays (two slots that share a page are not
+ * both written through in one call).  Where the cache has bounds, those of every block that
  * got a row are computed anew from the block's tokens up to the newest one written:
  *   lo = min, hi = max per channel of code * scale;  b = max |lo|, |hi|;  scale = b / 127;
  *   lo8 = max(-127, floor(lo * (127 / b))), hi8 = min(127, ceil(hi * (127 / b)));  scale +infinity if a row of the block has scale NaN
@@ -64,8 +65,8 @@ int qw_kv8_get(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *
 
 /* Attention of one new token per row over its slot's first lens[r] tokens: y = sum_t softmax_t(scale * q . k_t) v_t for each of the qh query heads
  * (qh / kvh = 1 .. 16 of them share a kv head, as consecutive ones), times sigmoid(gate) where there is a gate.  A row of length 0 is zero; a row with
- * a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks], distinct block numbers, the first
- * negative one ends them) the tokens are those of the named blocks.  An infinity or a NaN in a query makes its head's result NaN.
+ * a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks]: distinct block numbers in any order, then only negative ones, as pick
+ * leaves them) the tokens are those of the named blocks; a block beyond the row's last makes the head's result NaN.  An infinity or a NaN in a query makes its head's result NaN.
  * max_len: no row is longer (a longer one is answered with NaN).  What a row yields does not depend on the other rows of the call.
  * work: qw_kv8_attn_work(...) bytes, 16-byte aligned, nothing has to be in it. */
 typedef struct {
@@ -80,7 +81,8 @@ typedef struct {
     uint32_t nb, layer, dtype, qh, max_len, nblocks, reserved;   /* nb <= 1024 */
 } qw_kv8_attn_args;
 int qw_kv8_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, void *stream, char *err, size_t errlen);
-/* Workspace of attention over up to max_len tokens (or, with blocks, over nblocks of them); 0 for sizes the call would refuse. */
+/* Workspace of attention over up to max_len tokens; with nblocks, over that many blocks only (one for nblocks = 0 serves every list of blocks too).  0 for
+ * sizes the call would refuse. */
 size_t qw_kv8_attn_work(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_t max_len, uint32_t nblocks);
 
 /* The blocks of a row's context that are worth attending to, per kv head:  q8 = nearest(q * (127 / max |q|)), sq = max |q| / 127 per query head;

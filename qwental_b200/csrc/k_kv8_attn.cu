@@ -670,7 +670,9 @@ const char *check_shape(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_
     if (max_len < 1 || (uint64_t)max_len > (uint64_t)c->max_pages * KV8_PAGE) return "max_len is 1 to 256 max_pages";
     return nullptr;
 }
+// Without blocks: enough for lists of blocks as well, whose last block may reach beyond max_len.
 size_t work_of(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_t max_len, uint32_t nblocks) {
+    if (!nblocks) nblocks = (uint32_t)(((uint64_t)max_len + c->block - 1) / c->block);
     return (size_t)nb * chunks_of(c, max_len, nblocks) * qh * (c->hd + 2) * 4;
 }
 // 0, or -1 / -2 with a message

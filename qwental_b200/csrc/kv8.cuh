@@ -127,10 +127,5 @@ __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
 __device__ __forceinline__ void lds64(uint32_t &a, uint32_t &b, uint32_t addr) {
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
 
 }  // namespace qw

@@ -155,7 +155,7 @@ class Kv8Cache:
 
     # ---- calls
     def work_bytes(self, nb, qh, max_len, blocks=0):
-        """A workspace that serves attn (over everything, or over `blocks` chosen blocks) and pick for these sizes."""
+        """A workspace that serves pick and attn for these sizes, over everything or any list of blocks; given `blocks`, over lists of so many only."""
         n = self.L.qw_kv8_attn_work(C.byref(self.c), nb, qh, max_len, blocks)
         if n == 0:
             raise Kv8Error("sizes that the calls refuse")

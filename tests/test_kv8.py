@@ -149,6 +149,19 @@ def test_sizes_and_workspaces():
     assert L.qw_kv8_pick_work(C.byref(cache()), 2, 1000) >= 2 * 3 * 32 * 4 and L.qw_kv8_pick_work(C.byref(cache()), 2, 0) == 0
 
 
+@pytest.mark.parametrize("block", [16, 32, 64, 128, 256])
+def test_a_workspace_for_everything_serves_chosen_blocks(block):
+    """Blocks are gone over as a whole, so a list of them may need more chunks than the row's tokens: 70 tokens are three of 32, one block of 256 is eight."""
+    L = kv8.bind()
+    c = cache(block=block, pages=1000, max_pages=1000, layers=1)
+    for n in (1, 15, 16, 17, 70, 255, 256, 257, 500, 512, 513, 600, 2047, 2048, 2049, 2100, 65535, 65536, 65537, 70001):
+        w = L.qw_kv8_attn_work(C.byref(c), 2, 6, n, 0)
+        for k in (1, 2, 3, 5, 8, 100, 129, 4096, 1 << 20):
+            assert 0 < L.qw_kv8_attn_work(C.byref(c), 2, 6, n, k) <= w, (n, k)
+        assert call("qw_kv8_attn", c, attn(layer=0, max_len=n, work_bytes=w, blocks=4096, nblocks=-(-n // block)))[0] != -2
+        assert call("qw_kv8_attn", c, attn(layer=0, max_len=n, work_bytes=w))[0] != -2
+
+
 def test_rows_lie_where_the_layout_says_and_nothing_outside_is_touched():
     """The kernels' own index arithmetic (kv8.h), on the host."""
     L = kv8.bind()
