@@ -35,7 +35,7 @@ typedef struct {
     uint8_t *bounds;           /* NULL, or [pages][layers][kvh][256 / block][2 hd + 16], 16-byte aligned: lo int8[hd], hi int8[hd], fp32 scale, 12 unused */
     const int32_t *page_table; /* [slots][max_pages] page ids; entries past a slot's tokens are never looked at */
     uint32_t *status;          /* NULL, or a word the device can write */
-    uint32_t pages, layers, kvh; /* at most 2^31 - 1 rows: pages * layers * 2 * kvh * 256 */
+    uint32_t pages, layers, kvh; /* at most 32767 kv heads, and 2^31 - 1 rows: pages * layers * 2 * kvh * 256 */
     uint32_t hd;               /* 64, 128 or 256 */
     uint32_t format, block;    /* block: tokens per block of bounds and of chosen blocks: 16, 32, 64, 128 or 256 */
     uint32_t slots, max_pages;

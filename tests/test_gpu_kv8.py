@@ -210,6 +210,46 @@ def test_a_cache_without_bounds_stores_the_same_codes(hd, kvh):
     assert int(rig.status) & 0xf00 == 0x200
 
 
+@pytest.mark.parametrize("kvh,n", [(100, 300), (1, 256), (1, 257), (2, 128), (2, 129), (2, 1000), (300, 40)])
+def test_many_rows_at_once_and_one_by_one(kvh, n):
+    """Rows of several slots in mixed order, some for the same place, some not in use, in one call and one by one in the order of their positions: the same codes, scales and
+    bounds, however the call shares them out (few or many rows for the heads); a captured call leaves the same when it is replayed with other rows."""
+    block, slots, hd = 32, 5, 64
+    rng = np.random.default_rng(n)
+    cell = rng.permutation(slots * 256)[:n]
+    sl, ps = (cell // 256).astype(np.int32), (cell % 256).astype(np.int32)
+    sl[3::17], ps[5::19] = -1, -1
+    ps[n // 2], sl[n // 2] = ps[0], sl[0]  # the same place twice
+    x = [torch.from_numpy(rng.standard_normal((n, kvh, hd)).astype(np.float16)).cuda() for _ in range(2)]
+    idx = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+
+    def new():
+        t = [torch.zeros(slots, 1, 2, kvh, PAGE, hd, dtype=torch.uint8, device="cuda"), torch.zeros(slots, 1, 2, kvh, PAGE, device="cuda"),
+             torch.zeros(slots, 1, kvh, PAGE // block, 2 * hd + 16, dtype=torch.uint8, device="cuda")]
+        return t, kv8.Kv8Cache(t[0], t[1], torch.arange(slots, dtype=torch.int32, device="cuda").view(slots, 1), t[2], format="int8")
+
+    want, c = new()
+    for i in sorted(range(n), key=lambda i: (ps[i], i)):
+        c.put(x[0][i:i + 1], x[1][i:i + 1], idx(sl[i:i + 1]), idx(ps[i:i + 1]))
+    got, c = new()
+    c.put(x[0], x[1], idx(sl), idx(ps))
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    again, c = new()
+    s, p, k, v = torch.full((n,), -1, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros_like(x[0]), torch.zeros_like(x[1])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.put(k, v, s, p)
+    g.replay()  # no row is in use
+    assert not any(t.any() for t in again)
+    s.copy_(idx(sl)), p.copy_(idx(ps)), k.copy_(x[0]), v.copy_(x[1])
+    g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(again, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_rows_outside_the_cache_are_dropped_and_reported():
     rig = Rig([300], 2, 128, "int8", 64, layers=1, layer=0)
     n_slots = rig.table.shape[0]

@@ -44,7 +44,7 @@ def call(name, c, a):
 
 
 BAD_CACHE = [(dict(hd=96), "head dimension"), (dict(hd=0), "head dimension"), (dict(format=2), "format"), (dict(block=8), "block"), (dict(block=48), "block"),
-             (dict(block=512), "block"), (dict(pages=0), "at least one"), (dict(kvh=0), "at least one"), (dict(slots=0), "at least one"), (dict(max_pages=0), "at least one"),
+             (dict(block=512), "block"), (dict(pages=0), "at least one"), (dict(kvh=0), "at least one"), (dict(slots=0), "at least one"), (dict(kvh=32768, pages=1, layers=1), "kv heads"), (dict(max_pages=0), "at least one"),
              (dict(pages=1 << 21), "2^31"), (dict(layers=1 << 31, pages=1 << 31), "2^31"), (dict(max_pages=1 << 24), "2^31"), (dict(codes=None), "null pointer"), (dict(scales=None), "null pointer"),
              (dict(page_table=None), "null pointer"), (dict(codes=4097), "16-byte"), (dict(scales=4100), "16-byte"), (dict(bounds=4104), "16-byte")]
 
