@@ -3,8 +3,9 @@
 //   s_t = scale q . k_t          k_t = code * ks_t: the dot product of q and the codes, times ks_t
 //   y   = sum_t 2^(s'_t) vs_t code_t / sum_t 2^(s'_t),   s' = s log2(e)
 // A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with a running maximum M of s' + log2 vs, so that the weights of the codes are at
-// most 1 whatever the scales are; p_t = 2^(s'_t - M) is w_t / vs_t, at most 2^110.  A chunk leaves sum w_t code_t, M and l = sum p_t in fp32; the join is
-//   y = sum_c 2^(M_c - M*) acc_c / sum_c 2^(M_c - M*) l_c      with M* the maximum over the chunks, in the order of the chunks.
+// most 1 whatever the scales are (of a row of zeros, whose scale is 0, it is 0).  The denominator has a maximum of its own: l = sum 2^(s'_t - S) with S that of s',
+// since M may be far from S both ways, by as much as the scales of the values are from 1.  A chunk leaves acc = sum w_t code_t, M, S and l in fp32; the join is
+//   y = 2^(M* - S*) sum_c 2^(M_c - M*) acc_c / sum_c 2^(S_c - S*) l_c      with M*, S* the maxima over the chunks, in the order of the chunks.
 #include "kv8.cuh"
 #include "tmap.cuh"
 
@@ -18,13 +19,12 @@ namespace {
 __host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 65536 ? 7 : 8; }
 __host__ __device__ inline uint32_t chunk_of(uint32_t n) { return 1u << chunk_log(n); }
 __host__ __device__ inline uint32_t chunks_in(uint32_t n) { return (n + chunk_of(n) - 1) >> chunk_log(n); }
-constexpr float LOWEST = 7.7037197775489434e-34f, LOWEST_LOG2 = -110.f;  // 2^-110
 
 struct AttnArgs {
     const void *q, *gate;
     void *y;
     const int32_t *lens, *slots, *blocks;
-    float *part;  // [nb][max_chunks][qh][hd] sums of w code, then [nb][qh][max_chunks] of M, l
+    float *part;  // [nb][max_chunks][qh][hd] sums of w code, then [nb][qh][max_chunks] of M, S, l and one unused
     int64_t q_row, q_head, g_row, g_head, y_row, y_head;
     float scale2;  // softmax scale * log2(e)
     uint32_t nb, qh, G, max_len, nblocks, max_chunks;
@@ -51,17 +51,22 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x: 0 below 2^-126
     return y;
 }
 
-__device__ __forceinline__ float2 *stats_of(const AttnArgs &a, uint32_t hd, uint32_t r, uint32_t qh) {
-    return (float2 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
+__device__ __forceinline__ float4 *stats_of(const AttnArgs &a, uint32_t hd, uint32_t r, uint32_t qh) {
+    return (float4 *)(a.part + (size_t)a.nb * a.max_chunks * a.qh * hd) + ((size_t)r * a.qh + qh) * a.max_chunks;
 }
 
-// (M, l, acc) of some tokens joined with those of others
-__device__ __forceinline__ void join(float &M, float &l, float2 &acc, float M2, float l2, float2 acc2) {
-    const float m = fmaxf(M, M2), f = M == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(M - m), f2 = M2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : exp2f(M2 - m);  // (no maximum: nothing, or NaN)
-    M = m;
-    l = fmaf(l, f, l2 * f2);
-    acc.x = fmaf(acc.x, f, acc2.x * f2);
-    acc.y = fmaf(acc.y, f, acc2.y * f2);
+// What some tokens leave of two channels, joined with what others leave.  Where there is no maximum the sum is 0 or a NaN.
+struct Sums {
+    float M, S, l;
+    float2 acc;
+};
+__device__ __forceinline__ void join(Sums &x, float M, float S, float l, float2 acc) {
+    const float m = fmaxf(x.M, M), f = x.M == -INFINITY ? 1.f : exp2f(x.M - m), f2 = M == -INFINITY ? 1.f : exp2f(M - m);
+    const float n = fmaxf(x.S, S), g = x.S == -INFINITY ? 1.f : exp2f(x.S - n), g2 = S == -INFINITY ? 1.f : exp2f(S - n);
+    x.M = m, x.S = n;
+    x.l = fmaf(x.l, g, l * g2);
+    x.acc.x = fmaf(x.acc.x, f, acc.x * f2);
+    x.acc.y = fmaf(x.acc.y, f, acc.y * f2);
 }
 
 // ------------------------------------------------------------------------------------------------ core
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
     bool ok = true, more = true;
     uint32_t n = 0, have_r = 0xffffffffu, have_h = 0;
     uint32_t qf[NT][HD / 8];
-    float fac[NT][2], o[X::CH][NT][4], M[NT][2], l[NT][2];
+    float fac[NT][2], o[X::CH][NT][4], M[NT][2], S[NT][2], l[NT][2];  // S and l are of this lane's tokens alone until the chunk ends
     const uint32_t Kb = tiles_of(warp), Vb = Kb + KR * X::TILE;
     uint64_t *bars = bars_of(warp);
     auto load_queries = [&](uint32_t r, uint32_t h) {
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                 for (int x = 0; x < X::CH; x++) o[x][nt][0] = o[x][nt][1] = o[x][nt][2] = o[x][nt][3] = 0.f;
-                M[nt][0] = M[nt][1] = -INFINITY;
+                M[nt][0] = M[nt][1] = S[nt][0] = S[nt][1] = -INFINITY;
                 l[nt][0] = l[nt][1] = 0.f;
             }
         }
@@ -384,8 +389,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
             for (int e = 0; e < 2; e++) {
                 const float *sc = scales_of(warp) + sl * 2 * STEP + mt * 16 + g + 8 * e;
                 const float kscale = sc[0], vscale = sc[STEP];
-                // a scale below 2^-110, which put does not make, counts as 2^-110 here
-                lv[mt][e] = vscale < LOWEST ? LOWEST_LOG2 : __log2f(vscale);
+                lv[mt][e] = __log2f(vscale);  // -infinity for a row of zeros: no weight
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -462,11 +466,20 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 for (int d = 0; d < 2; d++) {
                     const float nm = fmaxf(M[nt][d], x1[nt][d]), f = M[nt][d] == -INFINITY ? 0.f : exp2_fast(M[nt][d] - nm);
                     M[nt][d] = nm;
-                    l[nt][d] *= f;
 #pragma unroll
                     for (int x = 0; x < X::CH; x++) o[x][nt][d] *= f, o[x][nt][2 + d] *= f;
                 }
         }
+        // ---- the denominator
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                const float nm = fmaxf(fmaxf(fmaxf(s[0][nt][d], s[0][nt][2 + d]), fmaxf(s[1][nt][d], s[1][nt][2 + d])), S[nt][d]);
+                const float at = nm == -INFINITY ? 0.f : nm;  // (nothing so far: every score is -infinity, or a NaN)
+                l[nt][d] = l[nt][d] * exp2_fast(S[nt][d] - at) + (exp2_fast(s[0][nt][d] - at) + exp2_fast(s[0][nt][2 + d] - at)) + (exp2_fast(s[1][nt][d] - at) + exp2_fast(s[1][nt][2 + d] - at));
+                S[nt][d] = nm;
+            }
         // ---- weights as B operands: [16 tokens][high parts of tokens 2t, 2t + 1, of 2t + 8, 2t + 9, then the remainders] of head g
         uint32_t p[2][NT][4];
 #pragma unroll
@@ -478,10 +491,8 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 for (int e = 0; e < 2; e++)
 #pragma unroll
                     for (int d = 0; d < 2; d++) {
-                        // (nothing so far: M is -infinity, and so is every score, or a NaN)
-                        const float off = s[mt][nt][2 * e + d] - (M[nt][d] == -INFINITY ? 0.f : M[nt][d]);
-                        l[nt][d] += exp2_fast(off);
-                        wt[2 * e + d] = exp2_fast(off + lv[mt][e]);
+                        // (no weight so far: M is -infinity, and so is every score or its value's log2, or one is a NaN)
+                        wt[2 * e + d] = exp2_fast(s[mt][nt][2 * e + d] - (M[nt][d] == -INFINITY ? 0.f : M[nt][d]) + lv[mt][e]);
                     }
                 const __half2 h01 = __floats2half2_rn(wt[0], wt[1]), h23 = __floats2half2_rn(wt[2], wt[3]);
                 const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
@@ -540,7 +551,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
         if (task.w & 2) {  // ---- the chunk's totals
             const size_t at = (size_t)task.x * a.max_chunks + task.z;
             float *dst = a.part + (at * a.qh + task.y * a.G + 2 * t) * HD + X::LANE * g;
-            float2 *st = stats_of(a, HD, task.x, task.y * a.G + 2 * t) + task.z;
+            float4 *st = stats_of(a, HD, task.x, task.y * a.G + 2 * t) + task.z;
             if (X::DUP) {
 #pragma unroll
                 for (int x = 0; x < X::CH; x++)
@@ -551,11 +562,14 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int d = 0; d < 2; d++) {
-                    float lt = l[nt][d];
+                    float sm = S[nt][d];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(0xffffffffu, sm, off));
+                    float lt = S[nt][d] == -INFINITY ? l[nt][d] : l[nt][d] * exp2_fast(S[nt][d] - sm);  // (0 or a NaN where there is no score)
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, off);
                     if (nt * 8 + 2 * t + d >= a.G) continue;
-                    if (g == 0) st[(nt * 8 + d) * a.max_chunks] = make_float2(M[nt][d], lt);
+                    if (g == 0) st[(nt * 8 + d) * a.max_chunks] = make_float4(M[nt][d], sm, lt, 0.f);
 #pragma unroll
                     for (int hf = 0; hf < X::HALVES; hf++)
 #pragma unroll
@@ -577,7 +591,8 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
 // per 64 channels, 7 this way), W = 4 for longer ones.  grid (8 / W) (head, row, 64 channels) per block of 256 (W = 1) or 1 per block of 128
 template <int HD, class T, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, AttnArgs a) {
-    __shared__ float2 part[W][32], stat[W];
+    __shared__ float2 part[W][32];
+    __shared__ float stat[W][3];
     pdl_sync();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x = W == 1 ? blockIdx.x * 8 + warp : blockIdx.x;
     const uint32_t ch = x % (HD / 64) * 64 + 2 * lane, y = x / (HD / 64), r = y / a.qh, qh = y % a.qh;
@@ -585,7 +600,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
     const int len = a.lens[r], slot = a.slots[r];
     if (slot < 0) return;
     const uint32_t nch = chunks_in(row_tokens(c, a, slot, len));
-    const float2 *st = stats_of(a, HD, r, qh);
+    const float4 *st = stats_of(a, HD, r, qh);
     const float *p = a.part + ((size_t)r * a.max_chunks * a.qh + qh) * HD + ch;
     const uint32_t cs = a.qh * HD;
     float2 gate = make_float2(0.f, 0.f);
@@ -593,15 +608,14 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
         const T *gp = (const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch;
         gate = make_float2(kv8_float(gp[0]), kv8_float(gp[1]));
     }
-    float M = -INFINITY, l = 0.f;
-    float2 acc = make_float2(0.f, 0.f);
+    Sums x0 = {-INFINITY, -INFINITY, 0.f, make_float2(0.f, 0.f)};
     for (uint32_t k0 = W == 1 ? 0 : 32 * warp; k0 < nch; k0 += 32 * W) {
-        const float2 s = k0 + lane < nch ? __ldcg(st + k0 + lane) : make_float2(-INFINITY, 0.f);
+        const float4 s = k0 + lane < nch ? __ldcg(st + k0 + lane) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
         float2 v[32];
 #pragma unroll
         for (uint32_t k = 0; k < 32; k++) v[k] = k0 + k < nch ? __ldcg((const float2 *)(p + (size_t)(k0 + k) * cs)) : make_float2(0.f, 0.f);
-        const float Mb = warp_max(s.x), w = s.x == -INFINITY ? 0.f : exp2f(s.x - Mb);
-        const float lb = warp_sum(s.x == -INFINITY ? s.y : s.y * w);  // (0, or NaN, where a chunk has no maximum)
+        const float M = warp_max(s.x), S = warp_max(s.y), w = s.x == -INFINITY ? 0.f : exp2f(s.x - M);
+        const float l = warp_sum(s.y == -INFINITY ? s.z : s.z * exp2f(s.y - S));  // (0, or NaN, where a chunk has no maximum)
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (uint32_t k = 0; k < 32; k++) {
@@ -609,20 +623,20 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
             sum.x = __fadd_rn(sum.x, __fmul_rn(v[k].x, wk));
             sum.y = __fadd_rn(sum.y, __fmul_rn(v[k].y, wk));
         }
-        join(M, l, acc, Mb, lb, sum);
+        join(x0, M, S, l, sum);
     }
     if (W > 1) {
-        part[warp % W][lane] = acc;
-        if (lane == 0) stat[warp % W] = make_float2(M, l);
+        part[warp % W][lane] = x0.acc;
+        if (lane == 0) stat[warp % W][0] = x0.M, stat[warp % W][1] = x0.S, stat[warp % W][2] = x0.l;
         __syncthreads();
         if (warp) return;
 #pragma unroll
-        for (int i = 1; i < W; i++) join(M, l, acc, stat[i].x, stat[i].y, part[i][lane]);
+        for (int i = 1; i < W; i++) join(x0, stat[i][0], stat[i][1], stat[i][2], part[i][lane]);
     }
     const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
-    const float f = bad ? __uint_as_float(0x7fffffffu) : l == 0.f ? 0.f : 1.f / l;
-    float out[2] = {acc.x * f, acc.y * f};
+    const float f = bad ? __uint_as_float(0x7fffffffu) : x0.l == 0.f ? 0.f : exp2f(x0.M - x0.S) / x0.l;
+    float out[2] = {x0.acc.x * f, x0.acc.y * f};
     if (a.gate) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));
     kv8_store<2>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, out);
 }
@@ -674,7 +688,7 @@ const char *check_shape(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_
 // Without blocks: enough for lists of blocks as well, whose last block may reach beyond max_len.
 size_t work_of(const qw_kv8_cache *c, uint32_t nb, uint32_t qh, uint32_t max_len, uint32_t nblocks) {
     if (!nblocks) nblocks = (uint32_t)(((uint64_t)max_len + c->block - 1) / c->block);
-    return (size_t)nb * chunks_of(c, max_len, nblocks) * qh * (c->hd + 2) * 4;
+    return (size_t)nb * chunks_of(c, max_len, nblocks) * qh * (c->hd + 4) * 4;
 }
 // 0, or -1 / -2 with a message
 int check_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, const char **m) {

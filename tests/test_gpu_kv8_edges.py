@@ -1,0 +1,103 @@
+"""Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from qwental_b200 import kv8  # noqa: E402
+from tests import kv8_ref as ref  # noqa: E402
+from tests.test_gpu_kv8 import PAGE, Rig, host  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+LN2 = np.log(2.0)
+
+
+def set_rows(rig, i, j, codes=None, scales=None, head=slice(None)):
+    """Keys (j = 0) or values (j = 1) of the first tokens of row i's slot: codes [n, hd], scales [n], for every head."""
+    n = len(codes if codes is not None else scales)
+    for p0 in range(0, n, PAGE):
+        p, m = rig.table[rig.slots[i], p0 // PAGE], min(PAGE, n - p0)
+        if codes is not None:
+            rig.codes[p, rig.layer, j, head, :m] = codes[p0:p0 + m].view(np.uint8)
+        if scales is not None:
+            rig.scales[p, rig.layer, j, head, :m] = scales[p0:p0 + m]
+
+
+def upload(rig):
+    rig.t["codes"].copy_(torch.from_numpy(rig.codes))
+    rig.t["scales"].copy_(torch.from_numpy(rig.scales))
+
+
+def one_code(fmt):
+    return 1 if fmt == "int8" else 0x38  # stands for 1
+
+
+def scored_by_channel_0(rig, i, s, fmt):
+    """Keys whose score with a query of ones in channel 0 is s[t], at softmax scale 1: one product each."""
+    codes = np.zeros((len(s), rig.hd), np.uint8)
+    codes[:, 0] = np.where(s < 0, 0xff if fmt == "int8" else 0xb8, one_code(fmt))
+    set_rows(rig, i, 0, codes, np.abs(s).astype(np.float32))
+
+
+def queries_of_channel_0(rig, n, heads, dtype):
+    q = torch.zeros(n, heads, rig.hd, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    return q
+
+
+# ------------------------------------------------------------------------------------------------ values that are zero, or far apart in size
+@pytest.mark.parametrize("fmt,dtype,value", [("int8", F16, 65504.0), ("e4m3", F16, 65504.0), ("int8", F16, 1e4), ("int8", F16, 1e3), ("int8", BF16, 1e6), ("e4m3", BF16, 1e30)])
+@pytest.mark.parametrize("n,zeros,hd,G", [(600, 32, 64, 2), (3000, 96, 128, 5), (3000, 32, 256, 12), (70000, 224, 64, 9)])
+def test_rows_of_zeros_before_large_values_count(n, zeros, hd, G, fmt, dtype, value):
+    """A row whose values are zero has its part of the softmax's sum, whatever comes later: tokens of zeros in the first steps of a chunk (of 2, 4 or 8 steps), then in
+    the chunk's last step one of a higher score and large values.
+    Tolerance: a score is one product, times the row's scale, the query's power of two and the softmax scale (three roundings of 2^-24), joined with log2 of the value's
+    scale (one more, and log2's own 2^-22) and a maximum (one more): 6 2^-24 (|s'| + |lv| + 15) + 2^-22 |lv| in the exponent, twice (a weight and the sum); exponentials
+    2^-22 each; sums and the join's products at most 300 roundings of 2^-23; then half a step of the result."""
+    wins = [0.0, 5.0, 7.5, 10.0, 13.0, 16.5, 25.0]  # by so much the large row's score is higher, in powers of two
+    chunk = 64 if n <= 2048 else 128 if n <= 65536 else 256
+    rig = Rig([n] * len(wins), 1, hd, fmt, layers=1, layer=0, seed=n)
+    v_one = rig.rng.integers(1, 120, hd).astype(np.uint8)
+    v_one[0] = 127 if fmt == "int8" else 0x7e  # the largest code
+    largest = ref.LARGEST[fmt]
+    vs = np.float32(value / largest)
+    for i, d in enumerate(wins):
+        s = np.full(n, -60.0)
+        s[chunk:chunk + zeros] = 0
+        s[2 * chunk - 1] = d * LN2
+        scored_by_channel_0(rig, i, s, fmt)
+        scales = np.full(n, vs * np.float32(2.0 ** -10), np.float32)
+        codes = np.tile(v_one, (n, 1))
+        scales[chunk:chunk + zeros] = 0
+        codes[chunk:chunk + zeros] = 0
+        scales[2 * chunk - 1] = vs
+        set_rows(rig, i, 1, codes, scales)
+    upload(rig)
+    q = queries_of_channel_0(rig, len(wins), G, dtype)
+    y = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=n, scale=1.0)
+    got = host(y).astype(np.float64)
+    for i, d in enumerate(wins):
+        k, v = rig.kv(i, 0)
+        want, _ = ref.attend(host(q)[i].astype(np.float64), k, v, 1.0)
+        lv = abs(np.log2(vs))
+        rel = 2 * LN2 * (6 * 2.0 ** -24 * (d + lv + 15) + 2.0 ** -22 * lv) + 2.0 ** -21 + 300 * 2.0 ** -23
+        tol = np.abs(want) * (rel + torch.finfo(dtype).eps / 2 * (1 + rel))
+        off = np.abs(got[i] - want)
+        assert (off <= tol).all(), (d, float((off / tol).max()), got[i, 0, :2], want[0, :2])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_a_row_of_nothing_but_zero_values_is_zero(fmt):
+    """300,000 tokens' worth of nothing: the sum of the weights stays a number (chunks of 256, 2^18 tokens and more)."""
+    n = 270_000
+    rig = Rig([16 * PAGE], 1, 64, fmt, layers=1, layer=0, seed=1)
+    rig.codes[:, :, 1] = 0
+    rig.scales[:, :, 1] = 0
+    upload(rig)
+    table = np.resize(rig.table[rig.slots[0], :16], (rig.table.shape[0], n // PAGE + 1)).astype(np.int32)
+    c = kv8.Kv8Cache(rig.t["codes"], rig.t["scales"], torch.from_numpy(table).cuda(), format=fmt)
+    q = rig.randn(1, 3, 64)
+    y = torch.full_like(q, 5.0)
+    c.attn(q, rig.idx([n]), rig.idx([0]), y, max_len=n)
+    assert (y == 0).all()
