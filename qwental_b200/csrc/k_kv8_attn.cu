@@ -78,7 +78,8 @@ __device__ __forceinline__ void join(Sums &x, float M, float S, float l, float2 
 //            lane takes 16 codes with one shared-memory load and they feed four products as they lie.
 //   values   O^T[16 channels][8 heads] += codes^T[16][16 tokens] . w^T     a lane takes 16 codes of four tokens; byte permutations pair the tokens; the weights
 //            change lanes by shuffles and travel as fp16 high part and remainder (22 bits), in two products, or, of up to four heads, in the columns of one.
-// Codes become fp16 numbers exactly (kv8.cuh), queries are divided by a power of two of their own first, so the products are exact and the sums fp32.
+// Codes become fp16 numbers exactly (kv8.cuh).  Queries go in as fp16 too, times the power of two that leaves a head's largest element in [2^15, 2^16): fp16 ones
+// stay what they are, bf16 ones too down to 2^-32 of the largest; smaller ones are rounded to 2^-40 of it.  The products are exact, their sums fp32.
 // Measured for 16 ragged rows of 1K to 48K tokens (210 MB, e4m3) against forms that were left: blocks of 8 warps that share a tile of 128 tokens, with two
 // barriers per tile, 87 us (scaling, maxima and barriers of a tile 2800 cycles, one after the other); e4m3 operands as they are (mma m16n8k32) no faster, that
 // product being converted to fp16 ones by the assembler at every use (19 cycles instead of 8).
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
     const uint32_t Kb = tiles_of(warp), Vb = Kb + KR * X::TILE;
     uint64_t *bars = bars_of(warp);
     auto load_queries = [&](uint32_t r, uint32_t h) {
-        // queries as B operands: lane (g, t) has head g, 16 channels of every 64, divided by a power of two that leaves the largest in [1, 2)
+        // queries as B operands: lane (g, t) has head g, 16 channels of every 64, times a power of two that leaves the largest in [2^15, 2^16)
         have_r = r, have_h = h;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -348,8 +349,8 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
             }
             m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const uint32_t ex = min(max(m >> 23, 1u), 253u);
-            const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+            const uint32_t ex = max(m >> 23, 16u);  // (so that the power and its inverse are normal numbers)
+            const float down = __uint_as_float((254u + 15u - ex) << 23), up = __uint_as_float((ex - 15u) << 23);
 #pragma unroll
             for (int x = 0; x < HD / 8; x++) {
                 const float2 f = kv8_float2<T>(qf[nt][x]);

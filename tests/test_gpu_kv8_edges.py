@@ -1,4 +1,5 @@
-"""Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size."""
+"""Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
+query far apart."""
 import numpy as np
 import pytest
 
@@ -101,3 +102,35 @@ def test_a_row_of_nothing_but_zero_values_is_zero(fmt):
     y = torch.full_like(q, 5.0)
     c.attn(q, rig.idx([n]), rig.idx([0]), y, max_len=n)
     assert (y == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ queries over a wide range
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,top,rest", [(F16, 60000.0, 0.05), (F16, 60000.0, 2e-4), (BF16, 1e4, 0.01), (BF16, 3e5, 1e-3), (BF16, 1e20, 1e12)])
+@pytest.mark.parametrize("hd,G", [(64, 7), (128, 2), (256, 16)])
+def test_small_elements_of_a_query_count_beside_a_large_one(hd, G, dtype, top, rest, fmt):
+    """One channel of the queries is far above the others and all keys are zero there, so that the others alone make the scores.
+    Values are not negative and every row of them has one channel, so a result's relative error is that of the weights: twice (hd + 8) 2^-23 of sum |q k| in the scores
+    (a weight and the sum), 2^-17 for exponentials, sums and log2 of the values' scales, then half a step of the result."""
+    n = 300
+    rig = Rig([n, 77], 1, hd, fmt, layers=1, layer=0, seed=hd + G)
+    rig.codes[:, :, 0, :, :, 5] = 0
+    for i in (0, 1):
+        m = int(rig.lens[i])
+        codes = np.zeros((m, hd), np.uint8)
+        codes[np.arange(m), np.arange(m) % hd] = rig.rng.integers(0x60, 0x7f, m)
+        set_rows(rig, i, 1, codes)
+    upload(rig)
+    q = rig.randn(2, G, hd, dtype=dtype, scale=rest)
+    q[:, :, 5] = top
+    y = torch.zeros_like(q)
+    sc = 2.0 / (rest * hd ** 0.5)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=n, scale=sc)
+    got, qn = host(y).astype(np.float64), host(q).astype(np.float64)
+    for i in (0, 1):
+        k, v = rig.kv(i, 0)
+        want, spread = ref.attend(qn[i], k, v, float(np.float32(sc)))
+        rel = 4 * (hd + 8) * 2.0 ** -23 * spread + 2.0 ** -17
+        tol = np.abs(want) * (rel + torch.finfo(dtype).eps / 2 * (1 + rel)) + 2.0 ** -25
+        off = np.abs(got[i] - want)
+        assert (off <= tol).all(), (i, float((off / tol).max()))
