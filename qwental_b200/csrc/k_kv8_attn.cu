@@ -2,9 +2,10 @@
 //
 //   s_t = scale q . k_t          k_t = code * ks_t: the dot product of q and the codes, times ks_t
 //   y   = sum_t 2^(s'_t) vs_t code_t / sum_t 2^(s'_t),   s' = s log2(e)
-// A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with a running maximum M of s' + log2 vs, so that the weights of the codes are at
-// most 1 whatever the scales are (of a row of zeros, whose scale is 0, it is 0).  The denominator has a maximum of its own: l = sum 2^(s'_t - S) with S that of s',
-// since M may be far from S both ways, by as much as the scales of the values are from 1.  A chunk leaves acc = sum w_t code_t, M, S and l in fp32; the join is
+// A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with M the running maximum of s' + log2 vs, less 15, so that the weights of the codes are at
+// most 2^15 whatever the scales are (of a row of zeros, whose scale is 0, it is 0).  They become two fp16 numbers, high part and remainder: 22 bits of a weight down to
+// 2^-16 of the largest one so far in the chunk, below that to 2^-40 of it.  The denominator has a maximum of its own: l = sum 2^(s'_t - S) with S that of s',
+// since M may be far from S both ways, by as much as the scales of the values are from 1.  (log2 and 2^x are the fast ones: 2^-22 of log2 vs, 2^-22 of a weight.)  A chunk leaves acc = sum w_t code_t, M, S and l in fp32; the join is
 //   y = 2^(M* - S*) sum_c 2^(M_c - M*) acc_c / sum_c 2^(S_c - S*) l_c      with M*, S* the maxima over the chunks, in the order of the chunks.
 #include "kv8.cuh"
 #include "tmap.cuh"
@@ -77,7 +78,7 @@ __device__ __forceinline__ void join(Sums &x, float M, float S, float l, float2 
 //   scores   S[16 tokens][8 heads] = codes[16][HD] . q^T     mma m16n8k16.  Which channel is which k of the product is free as long as both sides agree, so a
 //            lane takes 16 codes with one shared-memory load and they feed four products as they lie.
 //   values   O^T[16 channels][8 heads] += codes^T[16][16 tokens] . w^T     a lane takes 16 codes of four tokens; byte permutations pair the tokens; the weights
-//            change lanes by shuffles and travel as fp16 high part and remainder (22 bits), in two products, or, of up to four heads, in the columns of one.
+//            change lanes by shuffles and travel as fp16 high part and remainder, in two products, or, of up to four heads, in the columns of one.
 // Codes become fp16 numbers exactly (kv8.cuh).  Queries go in as fp16 too, times the power of two that leaves a head's largest element in [2^15, 2^16): fp16 ones
 // stay what they are, bf16 ones too down to 2^-32 of the largest; smaller ones are rounded to 2^-40 of it.  The products are exact, their sums fp32.
 // Measured for 16 ragged rows of 1K to 48K tokens (210 MB, e4m3) against forms that were left: blocks of 8 warps that share a tile of 128 tokens, with two
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int d = 0; d < 2; d++) {
-                x1[nt][d] = fmaxf(fmaxf(s[0][nt][d] + lv[0][0], s[0][nt][2 + d] + lv[0][1]), fmaxf(s[1][nt][d] + lv[1][0], s[1][nt][2 + d] + lv[1][1]));
+                x1[nt][d] = fmaxf(fmaxf(s[0][nt][d] + lv[0][0], s[0][nt][2 + d] + lv[0][1]), fmaxf(s[1][nt][d] + lv[1][0], s[1][nt][2 + d] + lv[1][1])) - 15.f;
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) x1[nt][d] = fmaxf(x1[nt][d], __shfl_xor_sync(0xffffffffu, x1[nt][d], off));
                 up |= x1[nt][d] > M[nt][d];

@@ -1,5 +1,5 @@
 """Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
-query far apart."""
+query far apart, weights far below the largest."""
 import numpy as np
 import pytest
 
@@ -104,7 +104,7 @@ def test_a_row_of_nothing_but_zero_values_is_zero(fmt):
     assert (y == 0).all()
 
 
-# ------------------------------------------------------------------------------------------------ queries over a wide range
+# ------------------------------------------------------------------------------------------------ queries and weights over a wide range
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype,top,rest", [(F16, 60000.0, 0.05), (F16, 60000.0, 2e-4), (BF16, 1e4, 0.01), (BF16, 3e5, 1e-3), (BF16, 1e20, 1e12)])
 @pytest.mark.parametrize("hd,G", [(64, 7), (128, 2), (256, 16)])
@@ -134,3 +134,57 @@ def test_small_elements_of_a_query_count_beside_a_large_one(hd, G, dtype, top, r
         tol = np.abs(want) * (rel + torch.finfo(dtype).eps / 2 * (1 + rel)) + 2.0 ** -25
         off = np.abs(got[i] - want)
         assert (off <= tol).all(), (i, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("below", [12, 20, 26, 28])
+@pytest.mark.parametrize("n,hd,G", [(200, 64, 3), (1500, 128, 8), (3000, 256, 11)])
+def test_weights_far_below_the_largest_count(n, hd, G, below):
+    """The first token of every chunk has almost all of the chunk's weight and values in channel 0 alone; the others, 2^-below of it each, have theirs in channel 1.
+    A weight w, the largest 2^15, is held as two fp16 numbers: to 2^-22 of itself, or to 2^-25 where that is more, so 2^-12 of itself at 2^-13 (28 below)."""
+    rig = Rig([n], 1, hd, "int8", layers=1, layer=0, seed=n)
+    chunk = 32 if n <= 512 else 64 if n <= 2048 else 128
+    s = np.full(n, -below * LN2)
+    s[::chunk] = 0
+    scored_by_channel_0(rig, 0, s, "int8")
+    codes = np.zeros((n, hd), np.uint8)
+    codes[:, 1] = 100
+    codes[::chunk] = 0
+    codes[::chunk, 0] = 100
+    set_rows(rig, 0, 1, codes, np.full(n, 0.25, np.float32))
+    upload(rig)
+    q = queries_of_channel_0(rig, 1, G, BF16)
+    y = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=n, scale=1.0)
+    k, v = rig.kv(0, 0)
+    want, _ = ref.attend(host(q)[0].astype(np.float64), k, v, 1.0)
+    rel = 2 * LN2 * 6 * 2.0 ** -24 * (below + 17) + max(2.0 ** -22, 2.0 ** (below - 40)) + 2.0 ** -16
+    off = np.abs(host(y)[0] - want)
+    assert (off <= np.abs(want) * (rel + 2.0 ** -8 * (1 + rel))).all(), (float((off / want.clip(1e-30)).max()), host(y)[0, 0, :2], want[0, :2])
+
+
+@pytest.mark.parametrize("hd,G,dtype", [(64, 4, F16), (128, 1, F16), (64, 8, F16), (256, 6, F16), (128, 16, F16)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_weights_are_held_to_more_than_eleven_bits(hd, G, dtype, fmt):
+    """Values of one size and both signs at almost equal weights, whose sum nearly cancels: what is left is far below the rounding of a weight to fp16.
+    Tolerance, of the value: exponents of at most 16, with three roundings of 2^-24 of a score of up to 1.5 and two more of 2^-24 of 16, times ln 2: 25.5 2^-24; an exponential
+    2^-22, a weight's two parts 2^-22, partial sums that stay below a few weights: under 2^-18 together.  With the high parts alone a weight is off by up to
+    2^-11, 2^-12.5 in the mean, and the sum by about 2^-12.5 / sqrt(40) = 2^-15.2."""
+    n = 40
+    rig = Rig([n], 1, hd, fmt, layers=1, layer=0, seed=hd)
+    s = rig.rng.uniform(0.2, 1.0, n // 2).repeat(2)
+    s[1::2] *= 1 + 2.0 ** -14
+    scored_by_channel_0(rig, 0, s, fmt)
+    codes = np.zeros((n, hd), np.uint8)
+    codes[0::2] = 100 if fmt == "int8" else 0x70
+    codes[1::2] = 256 - 100 if fmt == "int8" else 0xf0
+    set_rows(rig, 0, 1, codes, np.ones(n, np.float32))
+    upload(rig)
+    q = queries_of_channel_0(rig, 1, G, dtype)
+    q[0, :, 0] = 1 - torch.arange(G, device="cuda") / 32
+    y = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=n, scale=1.0)
+    k, v = rig.kv(0, 0)
+    want, _ = ref.attend(host(q)[0].astype(np.float64), k, v, 1.0)
+    off = np.abs(host(y)[0] - want)
+    assert np.abs(want).max() < 2.0 ** -12 * np.abs(v).max()
+    assert (off <= np.abs(v).max() * 2.0 ** -18 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all(), float(off.max() / np.abs(v).max())
