@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
     const float f = bad ? __uint_as_float(0x7fffffffu) : x0.l == 0.f ? 0.f : exp2f(x0.M - x0.S) / x0.l;
     float out[2] = {x0.acc.x * f, x0.acc.y * f};
-    if (a.gate) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));
+    if (a.gate && (bad || x0.l != 0.f)) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));  // (no token: zero, whatever the gate)
     kv8_store<2>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, out);
 }
 

@@ -1,5 +1,5 @@
 """Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
-query far apart, weights far below the largest."""
+query far apart, weights far below the largest; empty rows."""
 import numpy as np
 import pytest
 
@@ -188,3 +188,26 @@ def test_weights_are_held_to_more_than_eleven_bits(hd, G, dtype, fmt):
     off = np.abs(host(y)[0] - want)
     assert np.abs(want).max() < 2.0 ** -12 * np.abs(v).max()
     assert (off <= np.abs(v).max() * 2.0 ** -18 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all(), float(off.max() / np.abs(v).max())
+
+
+# ------------------------------------------------------------------------------------------------ results that are zero
+def test_an_empty_row_is_zero_whatever_its_gate_and_its_list_hold():
+    rig = Rig([0, 300, 0], 2, 128, "int8", 64, seed=3)
+    q, gate = rig.randn(3, 8, 128), rig.randn(3, 8, 128)
+    gate[0] = float("nan")
+    gate[2, 3] = float("-inf")
+    gate[1, 1, 7] = float("nan")  # of a row in use: its results are not numbers
+    blocks = np.tile(np.arange(6, dtype=np.int32), (3, 2, 1))
+    blocks[1, :, 5] = -1
+    for more in (dict(), dict(blocks=rig.idx(blocks))):
+        y = torch.full_like(q, 7.0)
+        rig.status.zero_()
+        rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, layer=1, max_len=300, gate=gate, **more)
+        assert (y[0] == 0).all() and (y[2] == 0).all() and y[1, 1, 7].isnan() and int(y[1].isnan().sum()) == 1 and int(rig.status) == 0
+
+
+def test_a_list_of_no_valid_blocks_is_zero_whatever_the_gate():
+    rig = Rig([300], 1, 64, "int8", 64, seed=3)
+    q, y = rig.randn(1, 2, 64), rig.randn(1, 2, 64)
+    rig.cache.attn(q, rig.idx([300]), rig.idx(rig.slots), y, layer=1, max_len=300, blocks=rig.idx(np.full((1, 1, 4), -1)), gate=torch.full_like(q, float("nan")))
+    assert (y == 0).all()
