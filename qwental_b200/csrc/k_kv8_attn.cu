@@ -637,9 +637,11 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
     }
     const bool bad = len > 0 && (uint32_t)len > a.max_len;
     if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
-    const float f = bad ? __uint_as_float(0x7fffffffu) : x0.l == 0.f ? 0.f : exp2f(x0.M - x0.S) / x0.l;
+    // a sum of nothing: no token, or scores of minus infinity alone
+    const bool none = x0.l == 0.f && (nch == 0 || (a.blocks && __ldcg(a.blocks + ((size_t)r * c.kvh + qh / a.G) * a.nblocks) < 0));
+    const float f = bad || (x0.l == 0.f && !none) ? __uint_as_float(0x7fffffffu) : none ? 0.f : exp2f(x0.M - x0.S) / x0.l;
     float out[2] = {x0.acc.x * f, x0.acc.y * f};
-    if (a.gate && (bad || x0.l != 0.f)) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));  // (no token: zero, whatever the gate)
+    if (a.gate && !none) out[0] *= 1.f / (1.f + expf(-gate.x)), out[1] *= 1.f / (1.f + expf(-gate.y));  // (no token: zero, whatever the gate)
     kv8_store<2>((T *)a.y + (int64_t)r * a.y_row + (int64_t)qh * a.y_head + ch, out);
 }
 

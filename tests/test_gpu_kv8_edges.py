@@ -1,5 +1,5 @@
 """Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
-query far apart, weights far below the largest; empty rows."""
+query far apart, weights far below the largest; empty rows, scores beyond the range."""
 import numpy as np
 import pytest
 
@@ -190,7 +190,7 @@ def test_weights_are_held_to_more_than_eleven_bits(hd, G, dtype, fmt):
     assert (off <= np.abs(v).max() * 2.0 ** -18 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all(), float(off.max() / np.abs(v).max())
 
 
-# ------------------------------------------------------------------------------------------------ results that are zero
+# ------------------------------------------------------------------------------------------------ results that are zero, and such that are no numbers
 def test_an_empty_row_is_zero_whatever_its_gate_and_its_list_hold():
     rig = Rig([0, 300, 0], 2, 128, "int8", 64, seed=3)
     q, gate = rig.randn(3, 8, 128), rig.randn(3, 8, 128)
@@ -211,3 +211,22 @@ def test_a_list_of_no_valid_blocks_is_zero_whatever_the_gate():
     q, y = rig.randn(1, 2, 64), rig.randn(1, 2, 64)
     rig.cache.attn(q, rig.idx([300]), rig.idx(rig.slots), y, layer=1, max_len=300, blocks=rig.idx(np.full((1, 1, 4), -1)), gate=torch.full_like(q, float("nan")))
     assert (y == 0).all()
+
+
+def test_scores_that_all_overflow_are_no_numbers():
+    """Scores of minus infinity alone leave nothing to divide by; one that is a number decides alone."""
+    rig = Rig([300, 300], 1, 64, "int8", layers=1, layer=0, seed=3)
+    for i in (0, 1):
+        s = np.full(300, -1e30)
+        if i:
+            s[123] = 0
+        scored_by_channel_0(rig, i, s, "int8")
+    upload(rig)
+    q = queries_of_channel_0(rig, 2, 3, BF16) * 1e20
+    blocks = rig.idx(np.tile(np.arange(5), (2, 1, 1)))
+    for more in (dict(), dict(blocks=blocks)):
+        y = torch.zeros_like(q)
+        rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=300, scale=1.0, **more)
+        assert y[0].isnan().all()
+        want = torch.from_numpy(rig.kv(1, 0)[1][123]).to(BF16)
+        assert (y[1].cpu().float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
