@@ -610,6 +610,14 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
         const T *gp = (const T *)a.gate + (int64_t)r * a.g_row + (int64_t)qh * a.g_head + ch;
         gate = make_float2(kv8_float(gp[0]), kv8_float(gp[1]));
     }
+    bool over = false;  // the core reads as many entries of a list as the row has blocks: further ones name none of them
+    if (a.blocks && nch && warp % W == 0) {
+        const int32_t *list = a.blocks + ((size_t)r * c.kvh + qh / a.G) * a.nblocks;
+#pragma unroll 8
+        for (uint32_t i = (min((uint32_t)len, a.max_len) + c.block - 1) / c.block + lane; i < a.nblocks; i += 32) over |= __ldcg(list + i) >= 0;
+        over = __any_sync(0xffffffffu, over);
+        if (over && lane == 0) set_status(c.status, ST_BAD_ARG | 0x23);
+    }
     Sums x0 = {-INFINITY, -INFINITY, 0.f, make_float2(0.f, 0.f)};
     for (uint32_t k0 = W == 1 ? 0 : 32 * warp; k0 < nch; k0 += 32 * W) {
         const float4 s = k0 + lane < nch ? __ldcg(st + k0 + lane) : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
@@ -635,8 +643,8 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, A
 #pragma unroll
         for (int i = 1; i < W; i++) join(x0, stat[i][0], stat[i][1], stat[i][2], part[i][lane]);
     }
-    const bool bad = len > 0 && (uint32_t)len > a.max_len;
-    if (bad && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
+    const bool longer = len > 0 && (uint32_t)len > a.max_len, bad = longer || over;
+    if (longer && lane == 0) set_status(c.status, ST_BAD_ARG | 0x24);
     // a sum of nothing: no token, or scores of minus infinity alone
     const bool none = x0.l == 0.f && (nch == 0 || (a.blocks && __ldcg(a.blocks + ((size_t)r * c.kvh + qh / a.G) * a.nblocks) < 0));
     const float f = bad || (x0.l == 0.f && !none) ? __uint_as_float(0x7fffffffu) : none ? 0.f : exp2f(x0.M - x0.S) / x0.l;

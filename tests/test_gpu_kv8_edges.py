@@ -1,5 +1,6 @@
 """Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
-query far apart, weights far below the largest; empty rows, scores beyond the range."""
+query far apart, weights far below the largest; empty rows, scores beyond the range, lists of blocks that are too
+long."""
 import numpy as np
 import pytest
 
@@ -230,3 +231,22 @@ def test_scores_that_all_overflow_are_no_numbers():
         assert y[0].isnan().all()
         want = torch.from_numpy(rig.kv(1, 0)[1][123]).to(BF16)
         assert (y[1].cpu().float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 256])
+def test_a_list_longer_than_its_row_has_blocks(block):
+    """A number beyond the row's last block is found wherever it stands in the list, in the head whose list it is; -1 behind the last is fine."""
+    n, kvh = 2 * block, 2
+    rig = Rig([n] * 6 + [3 * block - 5], kvh, 64, "e4m3", block, seed=2)
+    lists = [[0, 1, 7, -1], [7, 0, 1, -1], [0, -1, -1, 7], [1, 0, -1, -1], [0, 1, -1, 2], [0, 1, 0, -1], [2, 1, 0, 3]]
+    blocks = np.array([[x, [0, 1, -1, -1]] for x in lists], np.int32)
+    q = rig.randn(7, 2 * kvh, 64)
+    y = torch.zeros_like(q)
+    for r in range(7):
+        rig.status.zero_()
+        rig.cache.attn(q[r:r + 1], rig.idx([rig.lens[r]]), rig.idx(rig.slots[r:r + 1]), y[r:r + 1], layer=1, max_len=3 * block, blocks=rig.idx(blocks[r:r + 1]))
+        assert (int(rig.status) & 0xf00 == 0x200) == (r != 3), r
+        assert bool(y[r, :2].isnan().all()) == (r != 3) and y[r, 2:].isfinite().all(), r
+    many = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), many, layer=1, max_len=3 * block, blocks=rig.idx(blocks))
+    assert torch.equal(many.view(torch.int16), y.view(torch.int16))
