@@ -69,6 +69,7 @@ int qw_kv8_get(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *
  * then only negative ones, as pick leaves them) the tokens are those of the named blocks; a number beyond the row's last block makes the kv head's results
  * NaN, wherever it stands in the list.  An infinity or a NaN in a query makes its head's result NaN; so does a score beyond fp32's range, unless it is a
  * negative one beside others within it.
+ * y shares no memory with what the call reads, but it may be q itself, or the gate itself.
  * max_len: no row is longer (a longer one is answered with NaN).  What a row yields does not depend on the other rows of the call.
  * work: qw_kv8_attn_work(...) bytes, 16-byte aligned, nothing has to be in it. */
 typedef struct {

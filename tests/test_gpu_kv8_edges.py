@@ -1,6 +1,6 @@
 """Attention over the 8-bit key-value cache where its arithmetic can go wrong, against 64 bits: value rows that are zero or far apart in size, elements of a
-query far apart, weights far below the largest; empty rows, scores beyond the range, lists of blocks that are too
-long."""
+query far apart, weights far below the largest; rows in which every token and every chunk counts; empty rows, scores beyond the range, lists of
+blocks that are too long."""
 import numpy as np
 import pytest
 
@@ -191,6 +191,38 @@ def test_weights_are_held_to_more_than_eleven_bits(hd, G, dtype, fmt):
     assert (off <= np.abs(v).max() * 2.0 ** -18 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all(), float(off.max() / np.abs(v).max())
 
 
+# ------------------------------------------------------------------------------------------------ every token counts
+LONG = [31, 513, 2048, 2049, 4097, 5000, 8193, 20000, 48001, 65536, 65537, 70001]
+
+
+@pytest.mark.parametrize("hd,kvh,G,fmt,dtype,lens", [(256, 1, 8, "e4m3", F16, LONG), (256, 2, 3, "int8", F16, LONG), (256, 1, 16, "int8", BF16, LONG), (128, 1, 8, "int8", F16, LONG),
+                                                     (64, 1, 12, "e4m3", F16, [5000, 9001]), (128, 3, 1, "e4m3", F16, [20000]), (256, 1, 5, "int8", F16, [131073])])
+def test_every_token_of_a_long_row_counts(hd, kvh, G, fmt, dtype, lens):
+    """Token t has values in channel t % hd alone, and none are negative: a token, a step or a chunk that is lost, or counted twice, moves its channels by its share of
+    at least hd / tokens, and a result's relative error is that of its weights: in the scores twice (hd + 8) 2^-23 of sum |q k| (a weight and the sum), 2^-17 for
+    exponentials, log2, sums and joins; then half a step of the result."""
+    rig = Rig(lens, kvh, hd, fmt, layers=1, layer=0, seed=hd + G)
+    for i, n in enumerate(lens):
+        codes = np.zeros((n, hd), np.uint8)
+        codes[np.arange(n), np.arange(n) % hd] = rig.rng.integers(0x70, 0x7f, n)
+        set_rows(rig, i, 1, codes)
+    upload(rig)
+    qh = kvh * G
+    q = rig.randn(len(lens), qh, hd, dtype=dtype, scale=0.3)
+    y = torch.zeros_like(q)
+    rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, max_len=max(lens))
+    got, qn = host(y).astype(np.float64), host(q).astype(np.float64)
+    for i in range(len(lens)):
+        for h in range(kvh):
+            k, v = rig.kv(i, h)
+            g = slice(h * G, (h + 1) * G)
+            want, spread = ref.attend(qn[i, g], k, v, hd ** -0.5)
+            rel = 4 * (hd + 8) * 2.0 ** -23 * spread + 2.0 ** -17
+            tol = np.abs(want) * (rel + torch.finfo(dtype).eps / 2 * (1 + rel)) + 2.0 ** -25
+            off = np.abs(got[i, g] - want)
+            assert (off <= tol).all(), (lens[i], h, float((off / tol).max()))
+
+
 # ------------------------------------------------------------------------------------------------ results that are zero, and such that are no numbers
 def test_an_empty_row_is_zero_whatever_its_gate_and_its_list_hold():
     rig = Rig([0, 300, 0], 2, 128, "int8", 64, seed=3)
@@ -250,3 +282,15 @@ def test_a_list_longer_than_its_row_has_blocks(block):
     many = torch.zeros_like(q)
     rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), many, layer=1, max_len=3 * block, blocks=rig.idx(blocks))
     assert torch.equal(many.view(torch.int16), y.view(torch.int16))
+
+
+def test_results_in_place_of_the_queries_or_of_the_gate():
+    rig = Rig([0, 77, 700, 5000], 2, 128, "int8", seed=4)
+    q, gate = rig.randn(4, 8, 128), rig.randn(4, 8, 128)
+    y = torch.zeros_like(q)
+    call = lambda q, g, y: rig.cache.attn(q, rig.idx(rig.lens), rig.idx(rig.slots), y, layer=1, max_len=5000, gate=g)  # noqa: E731
+    call(q, gate, y)
+    a, b = q.clone(), gate.clone()
+    call(a, gate, a)
+    call(q, b, b)
+    assert torch.equal(a, y) and torch.equal(b, y)
