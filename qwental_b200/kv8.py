@@ -122,6 +122,8 @@ class Kv8Cache:
     def _blocks(self, t, nb):
         if t.dtype is not torch.int32 or t.dim() != 3 or t.shape[0] != nb or t.shape[1] != self.kvh or not t.is_contiguous() or t.get_device() != self.index:
             raise Kv8Error("blocks are int32 [%d, %d, n] on the cache's device" % (nb, self.kvh))
+        if t.shape[2] < 1:  # (its address is 0, which to the library is a call without a list)
+            raise Kv8Error("a list has room for one block at least")
         return t.data_ptr(), t.shape[2]
 
     def _work(self, work, need, stream):
