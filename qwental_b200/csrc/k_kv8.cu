@@ -351,6 +351,34 @@ bool kv8_aligned(int n2, int n4, const void *const *ptrs) {
         if ((uintptr_t)ptrs[i] & (i < n2 ? 1 : 3)) return false;
     return true;
 }
+static int64_t floor_div(int64_t x, int64_t y) { return x / y - (x % y && (x < 0)); }  // y > 0
+// Whether |d + i s1 + j s2| < hd for some |i| < n1 and |j| < n2; with `self` for others than i = j = 0.
+static bool meet(int64_t d, uint32_t n1, int64_t s1, uint32_t n2, int64_t s2, int64_t hd, bool self) {
+    const int64_t most = (int64_t)1 << 44;  // (no memory is that large: nothing below overflows)
+    auto size = [&](uint32_t n, int64_t s) { return n <= 1 ? 0 : s < -most || s > most ? most : s < 0 ? -s : s; };  // i and j take both signs
+    s1 = size(n1, s1), s2 = size(n2, s2);
+    if (s1 < s2) {
+        const int64_t s = s1;
+        const uint32_t n = n1;
+        s1 = s2, s2 = s, n1 = n2, n2 = n;
+    }
+    if (self && n2 > 1 && s2 == 0) return true;
+    int64_t from = -(int64_t)(n1 - 1), to = n1 - 1;  // of i, as far as the shorter stride can bridge the rest: a few where rows are apart
+    const int64_t reach = (n2 - 1) * s2 + hd - 1;
+    if (s1 > 0) {
+        const int64_t lo = floor_div(-reach - d, s1), hi = floor_div(reach - d, s1);
+        from = lo > from ? lo : from, to = hi < to ? hi : to;
+    }
+    for (int64_t i = from; i <= to; i++) {
+        const int64_t x = d + i * s1, j0 = s2 > 0 ? floor_div(-x, s2) : 0, last = n2 - 1;
+        for (int64_t j = j0; j <= j0 + 1; j++) {
+            const int64_t k = j < -last ? -last : j > last ? last : j, y = x + k * s2;
+            if (y < hd && y > -hd && !(self && i == 0 && k == 0)) return true;
+        }
+    }
+    return false;
+}
+bool kv8_overlap(uint32_t nb, uint32_t heads, uint32_t hd, int64_t row, int64_t head) { return meet(0, nb, row, heads, head, hd, true); }
 int kv8_fail(int code, const char *where, const char *msg, char *err, size_t errlen) {
     if (err && errlen) snprintf(err, errlen, "qw_%s: %s", where, msg);
     return code;

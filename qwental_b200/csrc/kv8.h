@@ -45,11 +45,8 @@ const char *kv8_check_layer(const qw_kv8_cache *c, uint32_t nb, uint32_t layer, 
 Kv8Dev kv8_dev(const qw_kv8_cache *c, uint32_t layer);
 // whether these pointers (nullptr ones pass) start at a boundary of their type: n2 of 2 bytes, then n4 of 4
 bool kv8_aligned(int n2, int n4, const void *const *ptrs);
-// whether different (row, head) of results would share bytes: a row's hd values are contiguous
-inline bool kv8_overlap(uint32_t nb, uint32_t heads, uint32_t hd, int64_t row, int64_t head) {
-    auto apart = [&](uint32_t n, int64_t s) { return n <= 1 || s >= (int64_t)hd || s <= -(int64_t)hd; };
-    return !apart(nb, row) || !apart(heads, head);
-}
+// whether two different (row, head) of results would share bytes: a row's hd values are contiguous, strides in elements
+bool kv8_overlap(uint32_t nb, uint32_t heads, uint32_t hd, int64_t row, int64_t head);
 int kv8_fail(int code, const char *where, const char *msg, char *err, size_t errlen);
 // nullptr, or why work on these pointers (nullptr ones are passed over) cannot be enqueued on the current device
 const char *kv8_check_device(const void *const *ptrs, int n);

@@ -23,3 +23,26 @@ def test_a_list_without_room_is_not_a_call_without_a_list():
         c.attn(x, i, i, x.clone(), max_len=10, blocks=none, work=work)
     with pytest.raises(kv8.Kv8Error, match="one block at least"):
         c.pick(x, i, i, none, max_len=10, first=0, last=0, work=work)
+
+
+def shares(nb, heads, hd, row, head):
+    """By going over every pair of results."""
+    at = sorted(int(x) for x in (np.arange(nb)[:, None] * row + np.arange(heads) * head).reshape(-1))
+    return any(b - a < hd for a, b in zip(at, at[1:]))
+
+
+def test_results_that_share_memory_are_refused_and_no_others():
+    """Row and head strides together: 128 and 128 put (row 0, head 1) where (row 1, head 0) is."""
+    rng = np.random.default_rng(3)
+    cases = [(2, 3, 128, 128), (2, 3, 256, 128), (2, 3, 384, 128), (2, 3, 128, 256), (2, 3, 300, 128), (2, 3, 383, 128), (2, 3, -384, 128), (2, 3, -256, 128), (5, 3, 128, 640), (5, 3, 128, 512),
+             (5, 3, 128, 639), (4, 3, 200, 400), (4, 3, 300, 450), (1, 3, 0, 128), (1, 3, 5, 128), (2, 3, 384, 0), (3, 3, 0, 384), (2, 3, 1 << 62, 128), (2, 3, -(1 << 63), 128), (1024, 3, 384, 128),
+             (1024, 3, 383, 128), (1024, 3, 128, 131072), (1024, 3, 128, 131071)]
+    cases += [(int(rng.integers(1, 12)), 3, int(rng.integers(-900, 900)), int(rng.integers(-900, 900))) for _ in range(3000)]
+    for heads in (1, 3, 6):  # (rows of three kv heads; results of one, three or six query heads)
+        for nb, _, row, head in cases if heads == 3 else cases[:23]:
+            want = "on one another" if shares(nb, heads, 128, row, head) else None
+            got = [call("qw_kv8_attn", cache(kvh=3 if heads > 1 else 1), attn(nb=nb, qh=heads, y_row=row, y_head=head))[1]]
+            if heads == 3:
+                got += [call("qw_kv8_get", cache(), rows(k=1 << 30, nb=nb, k_row=row, k_head=head, v_row=384, v_head=128))[1]]
+                got += [call("qw_kv8_get", cache(), rows(v=1 << 30, nb=nb, v_row=row, v_head=head, k_row=384, k_head=128))[1]]
+            assert all(("on one another" in m) == (want is not None) for m in got), (nb, heads, row, head, got)
