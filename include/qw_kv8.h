@@ -60,7 +60,7 @@ typedef struct {
  *   lo8 = max(-127, floor(lo * (127 / b))), hi8 = min(127, ceil(hi * (127 / b)));  scale +infinity if a row of the block has scale NaN
  * so a block's tokens are to be written in order (or together). */
 int qw_kv8_put(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *err, size_t errlen);
-/* Reads rows back: code * scale, rounded to the rows' type. */
+/* Reads rows back: code * scale, rounded to the rows' type.  No two results share memory; k and v of different strides do not lie between one another either. */
 int qw_kv8_get(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *err, size_t errlen);
 
 /* Attention of one new token per row over its slot's first lens[r] tokens: y = sum_t softmax_t(scale * q . k_t) v_t for each of the qh query heads

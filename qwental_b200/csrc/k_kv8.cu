@@ -288,6 +288,7 @@ int rows_call(const char *where, enqueue_rows f, const qw_kv8_cache *c, const qw
     if (m) return kv8_fail(-1, where, m, err, errlen);
     const void *ptrs[] = {c->codes, c->scales, c->bounds, c->page_table, c->status, a->k, a->v, a->slots, a->pos};
     if ((m = kv8_check_device(ptrs, 9))) return kv8_fail(-3, where, m, err, errlen);
+    if (f == enqueue_get && kv8_share(a, c->kvh, c->hd)) return kv8_fail(-1, where, "k and v lie on one another", err, errlen);
     qw_pdl_current_family(where);
     const cudaError_t e = f(c, a, (cudaStream_t)stream);
     if (e != cudaSuccess) return cudaGetLastError(), kv8_fail(-3, where, cudaGetErrorString(e), err, errlen);
@@ -301,7 +302,7 @@ cudaError_t rows_batch(const QwLaunch &L, enqueue_rows f) {
     QW_CHECK_ARG(kv8_from_binds(L, &c, &s) && L.has_bytes(8, 32));
     struct { int64_t s[4]; } st = L.bytes<decltype(st)>(8);
     const qw_kv8_rows a = {L.buf<void>(4), L.buf<void>(5), L.buf<int32_t>(6), L.buf<int32_t>(7), st.s[0], st.s[1], st.s[2], st.s[3], s.nb, s.layer, s.dtype, 0};
-    QW_CHECK_ARG(!check_rows(&c, &a) && (f != enqueue_get || !check_out(&c, &a)) && L.avail(6) >= (size_t)s.nb * 4 && L.avail(7) >= (size_t)s.nb * 4);
+    QW_CHECK_ARG(!check_rows(&c, &a) && (f != enqueue_get || (!check_out(&c, &a) && !kv8_share(&a, s.kvh, s.hd))) && L.avail(6) >= (size_t)s.nb * 4 && L.avail(7) >= (size_t)s.nb * 4);
     QW_CHECK_ARG(kv8_rows_fit(L, 4, s.nb, s.kvh, s.hd, a.k_row, a.k_head) && kv8_rows_fit(L, 5, s.nb, s.kvh, s.hd, a.v_row, a.v_head));
     return f(&c, &a, L.stream);
 }
@@ -379,6 +380,20 @@ static bool meet(int64_t d, uint32_t n1, int64_t s1, uint32_t n2, int64_t s2, in
     return false;
 }
 bool kv8_overlap(uint32_t nb, uint32_t heads, uint32_t hd, int64_t row, int64_t head) { return meet(0, nb, row, heads, head, hd, true); }
+bool kv8_share(const qw_kv8_rows *a, uint32_t heads, uint32_t hd) {
+    const double d = ((double)(intptr_t)a->k - (double)(intptr_t)a->v) / 2;
+    if (d > 1e17 || d < -1e17) return false;  // (addresses have 57 bits at most)
+    if ((a->nb <= 1 || a->k_row == a->v_row) && (heads <= 1 || a->k_head == a->v_head))
+        return meet(((intptr_t)a->k - (intptr_t)a->v) / 2, a->nb, a->k_row, heads, a->k_head, hd, false);
+    auto ends = [&](double row, double head, double &lo, double &hi) {
+        row *= a->nb - 1, head *= heads - 1;
+        lo = fmin(row, 0) + fmin(head, 0), hi = fmax(row, 0) + fmax(head, 0) + hd;
+    };
+    double klo, khi, vlo, vhi;
+    ends((double)a->k_row, (double)a->k_head, klo, khi);
+    ends((double)a->v_row, (double)a->v_head, vlo, vhi);
+    return d + klo < vhi && vlo < d + khi;
+}
 int kv8_fail(int code, const char *where, const char *msg, char *err, size_t errlen) {
     if (err && errlen) snprintf(err, errlen, "qw_%s: %s", where, msg);
     return code;

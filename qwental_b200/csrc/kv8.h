@@ -47,6 +47,8 @@ Kv8Dev kv8_dev(const qw_kv8_cache *c, uint32_t layer);
 bool kv8_aligned(int n2, int n4, const void *const *ptrs);
 // whether two different (row, head) of results would share bytes: a row's hd values are contiguous, strides in elements
 bool kv8_overlap(uint32_t nb, uint32_t heads, uint32_t hd, int64_t row, int64_t head);
+// whether k and v share bytes; where their strides differ, whether the memory between the first and the last of each does
+bool kv8_share(const qw_kv8_rows *a, uint32_t heads, uint32_t hd);
 int kv8_fail(int code, const char *where, const char *msg, char *err, size_t errlen);
 // nullptr, or why work on these pointers (nullptr ones are passed over) cannot be enqueued on the current device
 const char *kv8_check_device(const void *const *ptrs, int n);

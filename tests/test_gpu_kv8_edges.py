@@ -294,3 +294,31 @@ def test_results_in_place_of_the_queries_or_of_the_gate():
     call(a, gate, a)
     call(q, b, b)
     assert torch.equal(a, y) and torch.equal(b, y)
+
+
+# ------------------------------------------------------------------------------------------------ refusals that need a device
+def test_keys_and_values_are_not_read_back_into_one_place():
+    """k and v that share memory are refused before anything is launched; side by side, or in turn in one tensor, they are fine."""
+    n, kvh, hd = 5, 2, 64
+    rig = Rig([300], kvh, hd, "int8", layers=1, layer=0)
+    slots, pos = rig.idx(np.full(n, rig.slots[0])), rig.idx(np.arange(n) * 3)
+    flat = torch.zeros(8 * n * kvh * hd, dtype=torch.float16, device="cuda")
+    kw, vw = flat[:n * kvh * hd].view(n, kvh, hd), flat[n * kvh * hd:2 * n * kvh * hd].view(n, kvh, hd)
+    rig.cache.get(kw, vw, slots, pos)
+    want = kw.clone(), vw.clone()
+
+    def at(start, row, head):
+        return flat.as_strided((n, kvh, hd), (row, head, 1), start)
+
+    full = kvh * hd
+    for a, b in ((at(0, full, hd), at(0, full, hd)), (at(0, full, hd), at(hd - 1, full, hd)), (at(0, full, hd), at((n - 1) * full + hd, full, hd)), (at(0, 2 * full, hd), at(full - 1, 2 * full, hd)),
+                 (at(0, 2 * full, hd), at(2 * full - 1, 2 * full, hd)), (at(0, hd, n * hd), at(3 * hd + 1, hd, n * hd)), (at(0, full, hd), at(full, 2 * full, hd))):
+        flat.fill_(7)
+        with pytest.raises(kv8.Kv8Error, match="on one another"):
+            rig.cache.get(a, b, slots, pos)
+        assert (flat == 7).all()
+    for a, b in ((at(0, 2 * full, hd), at(full, 2 * full, hd)), (at(full, 2 * full, hd), at(0, 2 * full, hd)), (at(0, full, hd), at(n * full, full, hd)), (at(0, hd, 2 * n * hd), at(n * hd, hd, 2 * n * hd)),
+                 (at(0, 2 * full, 2 * hd), at(hd, 2 * full, 2 * hd)), (at(0, full, hd), at(n * full, 2 * full, hd))):
+        flat.fill_(7)
+        rig.cache.get(a, b, slots, pos)
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
