@@ -6,6 +6,7 @@ another stream than the call's is the caller's to record there.  Errors raise Kv
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -100,7 +101,7 @@ class Kv8Cache:
         ptr = [None if t is None else t.data_ptr() for t in self.tensors]
         self.c = CacheStruct(*ptr, pages, layers, kvh, hd, FORMATS[format], block or 64, page_table.shape[0], page_table.shape[1])
         self.kvh, self.hd, self.slots, self.max_pages = kvh, hd, page_table.shape[0], page_table.shape[1]
-        self._err = C.create_string_buffer(256)
+        self._local = threading.local()  # a buffer for messages per thread: the library writes it while other threads run
         self._ref = C.byref(self.c)
         if self.L.qw_kv8_bytes(C.byref(self.c), (C.c_size_t * 3)()):
             raise Kv8Error("a cache of these sizes is not supported (head dim 64, 128 or 256; blocks of 16 to 256 tokens)")
@@ -140,13 +141,16 @@ class Kv8Cache:
             raise Kv8Error("the cache is not in device memory (this library has no CPU path)")
         if stream is None:
             stream = _raw_stream(self.index)
+        err = getattr(self._local, "err", None)
+        if err is None:
+            err = self._local.err = C.create_string_buffer(256)
         if torch.cuda.current_device() == self.index:
-            rc = fn(self._ref, C.byref(args), stream, self._err, 256)
+            rc = fn(self._ref, C.byref(args), stream, err, 256)
         else:
             with torch.cuda.device(self.device):
-                rc = fn(self._ref, C.byref(args), stream, self._err, 256)
+                rc = fn(self._ref, C.byref(args), stream, err, 256)
         if rc:
-            raise Kv8Error(self._err.value.decode())
+            raise Kv8Error(err.value.decode())
 
     @staticmethod
     def _dtype(t, what):

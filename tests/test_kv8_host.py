@@ -1,5 +1,6 @@
 """The 8-bit key-value cache's host side without a GPU: arguments that would be taken for others, results that share memory, calls from several threads."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -46,3 +47,35 @@ def test_results_that_share_memory_are_refused_and_no_others():
                 got += [call("qw_kv8_get", cache(), rows(k=1 << 30, nb=nb, k_row=row, k_head=head, v_row=384, v_head=128))[1]]
                 got += [call("qw_kv8_get", cache(), rows(v=1 << 30, nb=nb, v_row=row, v_head=head, k_row=384, k_head=128))[1]]
             assert all(("on one another" in m) == (want is not None) for m in got), (nb, heads, row, head, got)
+
+
+def test_every_thread_gets_its_own_message(monkeypatch):
+    """Two threads in calls of one cache at the same time: a refusal's text is that of its own call, and a call that succeeds in between does not clear it."""
+    c, _, _ = on_cpu()
+    c.index = 0
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    meet, said = threading.Barrier(3), {}
+
+    def library(name, rc, late):  # stands in for a call that writes its message while others are under way
+        def f(ref, args, stream, err, size):
+            meet.wait(10)
+            if late:
+                meet.wait(10)
+            err.value = name.encode()
+            if not late:
+                meet.wait(10)
+            meet.wait(10)
+            return rc
+        return f
+
+    def run(name, rc, late):
+        try:
+            c._call(library(name, rc, late), kv8.RowsStruct(), 0)
+            said[name] = None
+        except kv8.Kv8Error as e:
+            said[name] = str(e)
+
+    threads = [threading.Thread(target=run, args=x) for x in (("first", -1, False), ("second", -1, True), ("", 0, True))]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert said == {"first": "first", "second": "second", "": None}
