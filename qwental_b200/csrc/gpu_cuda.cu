@@ -5,6 +5,7 @@
 #include "../../include/qw_gpu_ext.h"
 #include "qw_kern.h"
 
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -15,15 +16,17 @@
 #include <vector>
 
 // ------------------------------------------------------------------------------------------------ launch mode
-static int g_pdl = -1;
-static const char *g_pdl_family = "";
+static std::atomic<int> g_pdl{-1};
+static thread_local const char *g_pdl_family = "";  // launches are made from any thread
 void qw_pdl_current_family(const char *name) { g_pdl_family = name ? name : ""; }
 bool qw_pdl_enabled() {
-    if (g_pdl < 0) {
+    int on = g_pdl.load(std::memory_order_relaxed);
+    if (on < 0) {  // the first launch; what qw_set_pdl() says in the meantime stays
         const char *e = getenv("QW_PDL");
-        g_pdl = e ? (atoi(e) != 0) : 1;
+        const int want = e ? (atoi(e) != 0) : 1;
+        if (g_pdl.compare_exchange_strong(on, want)) on = want;
     }
-    if (!g_pdl) return false;
+    if (!on) return false;
     static const char *off = getenv("QW_PDL_OFF");  // comma-separated families launched without the attribute
     if (off && *g_pdl_family) {
         const size_t n = strlen(g_pdl_family);

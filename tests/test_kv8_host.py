@@ -1,5 +1,8 @@
 """The 8-bit key-value cache's host side without a GPU: arguments that would be taken for others, results that share memory, calls from several threads."""
 import ctypes as C
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -79,3 +82,25 @@ def test_every_thread_gets_its_own_message(monkeypatch):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert said == {"first": "first", "second": "second", "": None}
+
+
+def test_a_thread_launches_under_its_own_family():
+    """QW_PDL_OFF names families that are launched without the attribute; which one a launch is of is its thread's own."""
+    code = """
+import ctypes, threading
+from qwental_b200 import lib
+L = lib.load()
+family, enabled = L._Z21qw_pdl_current_familyPKc, L._Z14qw_pdl_enabledv
+family.argtypes, enabled.restype = [ctypes.c_char_p], ctypes.c_bool
+off, on = ctypes.create_string_buffer(b"kv8_get"), ctypes.create_string_buffer(b"kv8_put")
+family(off)
+assert not enabled()
+t = threading.Thread(target=lambda: (family(on), seen.append(enabled())))
+seen = []
+t.start()
+t.join()
+assert seen == [True] and not enabled(), (seen, enabled())
+"""
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, QW_PDL_OFF="kv8_get", QW_PDL="1"), capture_output=True, text=True, timeout=120,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(kv8.__file__))))
+    assert r.returncode == 0, r.stderr[-800:]
