@@ -132,7 +132,8 @@ __device__ __forceinline__ uint32_t scan_512(uint32_t v, uint32_t *ws, uint32_t 
 // two bits at a time with counters: 12.)  grid (kvh, nb) x 512
 constexpr uint32_t BEST_KEYS = 4096;
 __global__ void __launch_bounds__(512) kv8_best_k(Kv8Dev c, PickArgs a) {
-    __shared__ uint32_t hist[2048], ws[16], red[16][4], found[3], kept[BEST_KEYS];
+    __shared__ __align__(16) uint32_t hist[2048];  // (gone over in fours)
+    __shared__ uint32_t ws[16], red[16][4], found[3], kept[BEST_KEYS];
     pdl_sync();
     const uint32_t h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int len = a.lens[r], slot = a.slots[r];
