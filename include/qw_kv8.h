@@ -65,8 +65,8 @@ int qw_kv8_get(const qw_kv8_cache *c, const qw_kv8_rows *a, void *stream, char *
 
 /* Attention of one new token per row over its slot's first lens[r] tokens: y = sum_t softmax_t(scale * q . k_t) v_t for each of the qh query heads
  * (qh / kvh = 1 .. 16 of them share a kv head, as consecutive ones), times sigmoid(gate) where there is a gate.  A row of length 0 is zero, whatever its
- * gate and its list of blocks hold; a row with a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks]: distinct block numbers in any order,
- * then only negative ones, as pick leaves them) the tokens are those of the named blocks; a number beyond the row's last block makes the kv head's results
+ * gate and its list of blocks hold; a row with a negative slot stays as it was.  With `blocks` ([nb][kvh][nblocks]: up to 2^31 - 1 distinct block numbers in any
+ * order, then only negative ones, as pick leaves them) the tokens are those of the named blocks; a number beyond the row's last block makes the kv head's results
  * NaN, wherever it stands in the list.  An infinity or a NaN in a query makes its head's result NaN; so does a score beyond fp32's range, unless it is a
  * negative one beside others within it.
  * y shares no memory with what the call reads, but it may be q itself, or the gate itself.

@@ -708,6 +708,7 @@ int check_attn(const qw_kv8_cache *c, const qw_kv8_attn_args *a, const char **m)
     if ((*m = kv8_check_layer(c, a->nb, a->layer, a->dtype)) || (*m = check_shape(c, a->nb, a->qh, a->max_len))) return -1;
     if (!a->q || !a->y || !a->lens || !a->slots || !a->work) return *m = "null pointer argument", -1;
     if (a->blocks && a->nblocks < 1) return *m = "chosen blocks of no number", -1;
+    if (a->blocks && a->nblocks > KV8_MAX_BLOCKS) return *m = "a list holds at most 2^31 - 1 blocks", -1;
     const void *ptrs[] = {a->q, a->gate, a->y, a->lens, a->slots, a->blocks};
     if (!kv8_aligned(3, 3, ptrs)) return *m = "a tensor does not start at a boundary of its type", -1;
     if (kv8_overlap(a->nb, a->qh, c->hd, a->y_row, a->y_head)) return *m = "results that lie on one another", -1;

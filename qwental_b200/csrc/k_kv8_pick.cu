@@ -227,6 +227,7 @@ int check_pick(const qw_kv8_cache *c, const qw_kv8_pick_args *a, const char **m)
     if (a->qh < c->kvh || a->qh % c->kvh || a->qh / c->kvh > 16) return *m = "1 to 16 query heads share a kv head", -1;
     if (a->max_len < 1 || (uint64_t)a->max_len > (uint64_t)c->max_pages * KV8_PAGE) return *m = "max_len is 1 to 256 max_pages", -1;
     if (a->nblocks < 1 || (uint64_t)a->first + a->last > a->nblocks) return *m = "at least one block is chosen, and first + last of them at most", -1;
+    if (a->nblocks > KV8_MAX_BLOCKS) return *m = "a list holds at most 2^31 - 1 blocks", -1;
     if (!a->q || !a->lens || !a->slots || !a->blocks || !a->work) return *m = "null pointer argument", -1;
     const void *ptrs[] = {a->q, a->lens, a->slots, a->blocks};
     if (!kv8_aligned(1, 3, ptrs)) return *m = "a tensor does not start at a boundary of its type", -1;

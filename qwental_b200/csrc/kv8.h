@@ -5,6 +5,7 @@
 
 #define KV8_PAGE 256
 #define KV8_MAX_ROWS 1024  // rows of a call: a piece of a prompt
+#define KV8_MAX_BLOCKS 0x7fffffffu  // of a list: the kernels count its entries in 32 bits, in steps of up to 512
 #define KV8_TINY 7.8886090522101181e-31f  // 2^-100
 
 // What a kernel needs of a cache: one layer of it.

@@ -104,3 +104,14 @@ assert seen == [True] and not enabled(), (seen, enabled())
     r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, QW_PDL_OFF="kv8_get", QW_PDL="1"), capture_output=True, text=True, timeout=120,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(kv8.__file__))))
     assert r.returncode == 0, r.stderr[-800:]
+
+
+def test_a_list_of_more_blocks_than_are_counted_is_refused():
+    """Entries are counted in 32 bits, in steps of 32 or 512: with 2^32 - 1 of them a count would come round and never end."""
+    for n in (0x80000000, 0xfffffe00, 0xffffffff):
+        rc, m = call("qw_kv8_pick", cache(), pick(nblocks=n))
+        assert rc == -1 and "2^31 - 1 blocks" in m
+        rc, m = call("qw_kv8_attn", cache(), attn(blocks=4096, nblocks=n))
+        assert rc == -1 and "2^31 - 1 blocks" in m
+    for name, args in (("qw_kv8_pick", pick(nblocks=0x7fffffff)), ("qw_kv8_attn", attn(blocks=4096, nblocks=0x7fffffff)), ("qw_kv8_attn", attn(nblocks=0xffffffff))):
+        assert "blocks" not in call(name, cache(), args)[1]
