@@ -27,6 +27,12 @@ def _raw_stream(index):
     return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+def _in_32_bits(a, b=0, c=0, d=0):
+    """ctypes would cut larger or negative numbers down to 32 bits without a word."""
+    if not (0 <= a <= 0xffffffff and 0 <= b <= 0xffffffff and 0 <= c <= 0xffffffff and 0 <= d <= 0xffffffff):
+        raise Kv8Error("a layer, length or number of blocks, rows or heads that 32 bits do not hold")
+
+
 class CacheStruct(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "bounds", "page_table", "status")] + \
                [(n, C.c_uint32) for n in ("pages", "layers", "kvh", "hd", "format", "block", "slots", "max_pages")]
@@ -92,6 +98,7 @@ class Kv8Cache:
             block = PAGE // bounds.shape[3]
         if status is not None and (status.numel() < 1 or status.element_size() != 4):
             raise Kv8Error("status is one 32-bit word")
+        _in_32_bits(*page_table.shape)
         self.tensors = (codes, scales, bounds, page_table, status)
         self.device = codes.device
         self.index = codes.get_device()
@@ -125,6 +132,7 @@ class Kv8Cache:
             raise Kv8Error("blocks are int32 [%d, %d, n] on the cache's device" % (nb, self.kvh))
         if t.shape[2] < 1:  # (its address is 0, which to the library is a call without a list)
             raise Kv8Error("a list has room for one block at least")
+        _in_32_bits(t.shape[2])
         return t.data_ptr(), t.shape[2]
 
     def _work(self, work, need, stream):
@@ -162,6 +170,7 @@ class Kv8Cache:
     # ---- calls
     def work_bytes(self, nb, qh, max_len, blocks=0):
         """A workspace that serves pick and attn for these sizes, over everything or any list of blocks; given `blocks`, over lists of so many only."""
+        _in_32_bits(nb, qh, max_len, blocks)
         n = self.L.qw_kv8_attn_work(C.byref(self.c), nb, qh, max_len, blocks)
         if n == 0:
             raise Kv8Error("sizes that the calls refuse")
@@ -169,6 +178,7 @@ class Kv8Cache:
 
     def _rows_call(self, fn, k, v, slots, pos, layer, stream):
         nb, dt = slots.shape[0], self._dtype(k, "k")
+        _in_32_bits(nb, layer)
         kp, kr, kh = self._rows(k, nb, self.kvh, k.dtype, "k")
         vp, vr, vh = self._rows(v, nb, self.kvh, k.dtype, "v")
         self._call(fn, RowsStruct(kp, vp, self._index(slots, nb, "slots"), self._index(pos, nb, "pos"), kr, kh, vr, vh, nb, layer, dt), stream)
@@ -184,6 +194,7 @@ class Kv8Cache:
     def attn(self, q, lens, slots, y, layer=0, *, max_len, scale=None, gate=None, blocks=None, work=None, stream=None):
         """y [nb, qh, hd] = attention of q over the first lens[r] tokens of slot slots[r] (of the blocks [nb, kvh, n], if given), times sigmoid(gate)."""
         nb, qh, dt = lens.shape[0], q.shape[1] if q.dim() == 3 else 0, self._dtype(q, "q")
+        _in_32_bits(nb, qh, layer, max_len)
         qp, qr, qd = self._rows(q, nb, qh, q.dtype, "q")
         yp, yr, yd = self._rows(y, nb, qh, q.dtype, "y")
         gp, gr, gd = (None, 0, 0) if gate is None else self._rows(gate, nb, qh, q.dtype, "gate")
@@ -196,6 +207,8 @@ class Kv8Cache:
     def pick(self, q, lens, slots, blocks, layer=0, *, max_len, first=0, last=1, work=None, stream=None):
         """blocks [nb, kvh, n]: the block numbers with the best scores for q, ascending, the first `first` and the last `last` always among them."""
         nb, qh, dt = lens.shape[0], q.shape[1] if q.dim() == 3 else 0, self._dtype(q, "q")
+        _in_32_bits(nb, qh, layer, max_len)
+        _in_32_bits(first, last)
         qp, qr, qd = self._rows(q, nb, qh, q.dtype, "q")
         bp, nblocks = self._blocks(blocks, nb)
         work, wp, size = self._work(work, self.L.qw_kv8_pick_work(self._ref, nb, max_len) if work is None else 0, stream)

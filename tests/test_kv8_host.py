@@ -115,3 +115,25 @@ def test_a_list_of_more_blocks_than_are_counted_is_refused():
         assert rc == -1 and "2^31 - 1 blocks" in m
     for name, args in (("qw_kv8_pick", pick(nblocks=0x7fffffff)), ("qw_kv8_attn", attn(blocks=4096, nblocks=0x7fffffff)), ("qw_kv8_attn", attn(nblocks=0xffffffff))):
         assert "blocks" not in call(name, cache(), args)[1]
+
+
+@pytest.mark.parametrize("bad", [1 << 32, (1 << 32) + 10, -1, -(1 << 32) + 10, 1 << 64])
+def test_numbers_that_32_bits_do_not_hold_are_refused(bad):
+    """They would arrive as others: a max_len of 2^32 + 10 as 10, layer 2^32 as layer 0."""
+    c, x, i = on_cpu()
+    ids, work = torch.zeros(2, 2, 3, dtype=torch.int32), torch.zeros(1 << 20, dtype=torch.uint8)
+    calls = [lambda: c.put(x, x, i, i, layer=bad), lambda: c.get(x, x.clone(), i, i, layer=bad), lambda: c.attn(x, i, i, x.clone(), max_len=bad, work=work),
+             lambda: c.attn(x, i, i, x.clone(), layer=bad, max_len=10, work=work), lambda: c.attn(x, i, i, x.clone(), max_len=bad),
+             lambda: c.pick(x, i, i, ids, max_len=bad, work=work), lambda: c.pick(x, i, i, ids, layer=bad, max_len=10, work=work), lambda: c.pick(x, i, i, ids, max_len=10, first=bad, work=work),
+             lambda: c.pick(x, i, i, ids, max_len=10, last=bad, work=work), lambda: c.work_bytes(bad, 2, 10), lambda: c.work_bytes(1, bad, 10), lambda: c.work_bytes(1, 2, bad),
+             lambda: c.work_bytes(1, 2, 10, bad)]
+    for f in calls:
+        with pytest.raises(kv8.Kv8Error, match="32 bits"):
+            f()
+
+
+def test_a_page_table_that_32_bits_do_not_hold_is_refused():
+    meta = lambda *s, dtype=torch.uint8: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    for shape in ((1, (1 << 32) + 5), ((1 << 32) + 5, 1)):
+        with pytest.raises(kv8.Kv8Error, match="32 bits"):
+            kv8.Kv8Cache(meta(3, 1, 2, 2, 256, 64), meta(3, 1, 2, 2, 256, dtype=torch.float32), meta(*shape, dtype=torch.int32))
