@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
     load_queries(f.r, f.h);  // the first task's, while its tile is on its way
     for (; more; n++) {
         const uint32_t sl = n % KR, vl = n % VR;
-        if (!mbar_wait(&bars[KF + sl], n / KR & 1)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars[KF + sl], n / KR & 1))) {  // (the warp gives up as a whole: its lanes need one another below)
             ok = false;
             break;
         }
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 if (X::DUP) p[mt][nt][0] = to_b(t < 2 ? h01 : r01), p[mt][nt][1] = to_b(t < 2 ? h23 : r23);  // columns 4 to 7 are the same heads: their remainders
                 else p[mt][nt][0] = to_b(h01), p[mt][nt][1] = to_b(h23), p[mt][nt][2] = to_b(r01), p[mt][nt][3] = to_b(r23);
             }
-        if (!mbar_wait(&bars[VF + vl], n / VR & 1)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars[VF + vl], n / VR & 1))) {
             ok = false;
             break;
         }
