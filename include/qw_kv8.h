@@ -15,7 +15,8 @@
  * nothing was enqueued, unless the code is -3.
  *
  * Slots, positions and page ids are device data, so the kernels check them: a slot or page outside the cache is never read or written; the row's
- * results are NaN (put: the row is dropped; pick: -1), and the word at `status`, if there is one, becomes 0x200 | n.
+ * results are NaN (put: the row is dropped; pick: -1), and the word at `status`, if there is one, becomes 0x200 | n.  Attention whose copies do not arrive
+ * within two seconds gives up: the rows concerned are NaN, and the word becomes 0x100 | n.
  */
 #ifndef QW_KV8_H
 #define QW_KV8_H

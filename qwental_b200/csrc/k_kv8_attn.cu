@@ -85,6 +85,10 @@ __device__ __forceinline__ void join(Sums &x, float M, float S, float l, float2 
 // barriers per tile, 87 us (scaling, maxima and barriers of a tile 2800 cycles, one after the other); e4m3 operands as they are (mma m16n8k32) no faster, that
 // product being converted to fp16 ones by the assembler at every use (19 cycles instead of 8).
 constexpr uint32_t STEP = 32;
+__device__ __forceinline__ uint32_t share_start(uint32_t total, uint32_t w, uint32_t W) {  // total w / W, in 32 bits
+    const uint32_t per = total / W, rest = total - per * W;
+    return w * per + w * rest / W;
+}
 
 template <int HD, int MODE, bool FEW>
 struct Core {
@@ -105,8 +109,26 @@ struct Core {
     static_assert(WARPS + 1 <= 16 && BYTES + 12 * KV8_MAX_ROWS <= 227 * 1024, "words of HAS, and what a block may have");
 };
 
+// Of a warp that gave up: what its share of the tasks leaves is not numbers, nor are the rows they are part of, whatever the workspace held.  A function of its own, so that
+// nothing is kept for it in the registers of the loop.
+__device__ __noinline__ void void_share(const Kv8Dev &c, const AttnArgs &a, const uint32_t *first, uint32_t w, uint32_t W, uint32_t hd) {
+    __syncwarp();  // (behind what it may have left already)
+    const uint32_t lane = threadIdx.x & 31, total = first[a.nb] * c.kvh, lo = share_start(total, w, W), hi = share_start(total, w + 1, W);
+    for (uint32_t r = 0; r < a.nb; r++) {
+        const uint32_t steps = first[r + 1] - first[r];
+        if (!steps) continue;
+        const uint32_t n = row_tokens(c, a, a.slots[r], a.lens[r]), cs = chunk_of(n) / STEP, chunks = chunks_in(n);
+        for (uint32_t i = lane; i < c.kvh * chunks; i += 32) {
+            const uint32_t h = i / chunks, ch = i % chunks, at = first[r] * c.kvh + h * steps + ch * cs;
+            if (at >= lo && at < hi)
+                for (uint32_t g = 0; g < a.G; g++) stats_of(a, hd, r, h * a.G + g)[ch] = make_float4(-INFINITY, -INFINITY, __uint_as_float(0x7fffffffu), 0.f);
+        }
+    }
+}
+
 template <int HD, int FMT, class T, int MODE, bool FEW>
-__global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(const __grid_constant__ CUtensorMap tm, Kv8Dev c, AttnArgs a, uint32_t box_rows, unsigned *status) {
+__global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(const __grid_constant__ CUtensorMap tm, const __grid_constant__ Kv8Dev c, const __grid_constant__ AttnArgs a, uint32_t box_rows,
+                                                                                 unsigned *status) {
     typedef Core<HD, MODE, FEW> X;
     constexpr int KR = X::KR, VR = X::VR, NT = X::NT;
     extern __shared__ uint8_t smem_raw[];
@@ -184,7 +206,7 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
     auto find = [&](uint32_t w) {  // warp w's; returns the end of its share
         // few tasks go to different SMs first; many to neighbours, who mostly read the same queries
         const uint32_t W = gridDim.x * X::WARPS, w0 = FEW ? w * gridDim.x + blockIdx.x : blockIdx.x * X::WARPS + w;
-        const uint32_t per = total / W, rest = total - per * W, lo = w0 * per + w0 * rest / W, hi = (w0 + 1) * per + (w0 + 1) * rest / W;  // (total w / W, in 32 bits)
+        const uint32_t lo = share_start(total, w0, W), hi = share_start(total, w0 + 1, W);
         f.at = total;
         if (lo < hi) {
             uint32_t l = 0, u = a.nb;  // the last row that starts at or before lo
@@ -582,7 +604,10 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
                 }
         }
     }
-    if (!ok && lane == 0) set_status(status, ST_MBAR_TIMEOUT | 0x23);
+    if (!ok) {
+        if (lane == 0) set_status(status, ST_MBAR_TIMEOUT | 0x23);
+        void_share(c, a, first, FEW ? warp * gridDim.x + blockIdx.x : blockIdx.x * X::WARPS + warp, gridDim.x * X::WARPS, HD);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ join
