@@ -42,7 +42,8 @@ __device__ __forceinline__ void quantise_row(const Kv8Dev &c, size_t row, const 
     if (lane == 0) c.scales[row] = nan ? __uint_as_float(0x7fffffffu) : zero ? 0.f : __fdiv_rn(am, F);
 }
 
-// A cache without bounds: a warp per (row, head, K or V).  Bound: 6 bytes per value pass, 3.1 MB for 1024 rows of the benchmark's layer.  grid nb x 256
+// A cache without bounds: a warp per (row, head, K or V).  Bound: the latency of slot, page, a look at all later rows for the same position, and values; per call in a
+// captured graph 16 rows (hd 256, 2 kv heads) 1.9 us, 419 (hd 128, 8 kv heads) 4.7, 1024 (hd 256, 2 kv heads; 3.1 MB) 4.2.  grid nb x 256
 template <int HD, int FMT, class T>
 __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
     constexpr int E = HD / 32;
@@ -71,7 +72,8 @@ __global__ void __launch_bounds__(256) kv8_put_k(Kv8Dev c, RowArgs a) {
 // block and newer (most rows of a prompt are not), and leads if no other row is.  Keys (with the bounds) and values are different blocks of threads.
 // Bound: the latency of one after the other: rows' numbers, their values, the block's keys from L2.  From a captured graph, per call: 16 rows (hd 256, 2 kv heads) 5.4 us, 419
 // (hd 128, 8 kv heads) 7.1, 1024 (hd 256, 2 kv heads) 8.9; with the search in global memory and keys and values in the same block 5.3, 14.5 and 14.3; with that list of
-// rows for calls of a row per block of threads too, 6.2 for the 16.
+// rows for calls of a row per block of threads too, 6.2 for the 16.  Work is shared out by blocks of the cache: 1024 rows with blocks of 256 and one kv head (hd 256) are five
+// leaders for keys and for values each, and take 18.3 us; with blocks of 16 and eight kv heads (hd 128) 13.3.
 // grid (blocks of threads that share the leaders, 2 kvh) x 512
 template <int HD, int FMT, class T>
 __global__ void __launch_bounds__(512, 2) kv8_put_blocks_k(Kv8Dev c, RowArgs a) {

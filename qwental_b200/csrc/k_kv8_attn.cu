@@ -5,7 +5,8 @@
 // A value's scale goes into the exponent, w_t = 2^(s'_t + log2 vs_t - M) with M the running maximum of s' + log2 vs, less 15, so that the weights of the codes are at
 // most 2^15 whatever the scales are (of a row of zeros, whose scale is 0, it is 0).  They become two fp16 numbers, high part and remainder: 22 bits of a weight down to
 // 2^-16 of the largest one so far in the chunk, below that to 2^-40 of it.  The denominator has a maximum of its own: l = sum 2^(s'_t - S) with S that of s',
-// since M may be far from S both ways, by as much as the scales of the values are from 1.  (log2 and 2^x are the fast ones: 2^-22 of log2 vs, 2^-22 of a weight.)  A chunk leaves acc = sum w_t code_t, M, S and l in fp32; the join is
+// since M may be far from S both ways, by as much as the scales of the values are from 1.  (log2 and 2^x are the fast ones: 2^-22 of log2 vs, 2^-22 of a weight.)  A chunk
+// leaves acc = sum w_t code_t, M, S and l in fp32; the join is
 //   y = 2^(M* - S*) sum_c 2^(M_c - M*) acc_c / sum_c 2^(S_c - S*) l_c      with M*, S* the maxima over the chunks, in the order of the chunks.
 #include "kv8.cuh"
 #include "tmap.cuh"
@@ -15,7 +16,8 @@ using namespace qw;
 namespace {
 // Tokens of a chunk, by the tokens of its row alone (a row's result does not depend on the others of a call): short rows in small pieces, for their latency;
 // a chunk of 128 leaves 12 % of its own bytes as fp32 sums, in L2.  With 256 from 8193 tokens on, one row of 48000 took 24 us instead of 20 and 16 ragged rows
-// of 1K to 48K had single warps that ended 9 us after the others.
+// of 1K to 48K had single warps that ended 9 us after the others; beyond 65536 a warp has chunks enough, and half the sums to join count for more: one row of 131000 takes 42 us
+// instead of 53, of 500000 135 instead of 163, 8 rows of 70K to 130K 163 instead of 179 (one of 66000, just behind the step, 33 instead of 29.5).
 // Twice as many for more than eight heads, whose sums are larger, gained 4 to 8 % where there were many rows of up to 2048 tokens and lost 20 to 30 % in most other calls.
 __host__ __device__ inline uint32_t chunk_log(uint32_t n) { return n <= 512 ? 5 : n <= 2048 ? 6 : n <= 65536 ? 7 : 8; }
 __host__ __device__ inline uint32_t chunk_of(uint32_t n) { return 1u << chunk_log(n); }
@@ -84,6 +86,8 @@ __device__ __forceinline__ void join(Sums &x, float M, float S, float l, float2 
 // Measured for 16 ragged rows of 1K to 48K tokens (210 MB, e4m3) against forms that were left: blocks of 8 warps that share a tile of 128 tokens, with two
 // barriers per tile, 87 us (scaling, maxima and barriers of a tile 2800 cycles, one after the other); e4m3 operands as they are (mma m16n8k32) no faster, that
 // product being converted to fp16 ones by the assembler at every use (19 cycles instead of 8).
+// Bound: 46 us (4.6 TB/s, 0.7 of the copy rate): 5 us before a first tile, a tail of 7; ALU pipe 29 %, tensor pipe 21 %, issue slots 25 %.  Nine to sixteen heads at hd 256: latency of
+// seven warps per SM at 255 registers, about 300 bytes of them spilled (10 rows of 1612 tokens, 128 heads on 8: 34 us; issue slots 17 %, DRAM 20 %).
 constexpr uint32_t STEP = 32;
 __device__ __forceinline__ uint32_t share_start(uint32_t total, uint32_t w, uint32_t W) {  // total w / W, in 32 bits
     const uint32_t per = total / W, rest = total - per * W;
@@ -614,8 +618,8 @@ __global__ void __launch_bounds__(Core<HD, MODE, FEW>::THREADS, 1) kv8_attn_k(co
 // 64 channels of a (head, row): two channels per lane.  A warp takes 32 chunks at a time, a lane knows one chunk's weight (within the 32: relative to their
 // maximum) and every load leaves before the weights are known; the 32 are added in order, then joined with what the warp has.  W warps take every Wth 32 and are
 // joined in order, so a row's result depends on its own chunks alone, and up to 32 chunks W does not matter.  Rows of length 0 get their zeros here.
-// Bound: the latency of a few loads one after the other.  W = 1 for calls of up to 32 chunks (4096 (head, row) pairs of 32 chunks: 16 us in blocks of 256 threads
-// per 64 channels, 7 this way), W = 4 for longer ones.  grid (8 / W) (head, row, 64 channels) per block of 256 (W = 1) or 1 per block of 128
+// Bound: the latency of a few loads one after the other.  W = 1 for calls of up to 32 chunks (2048 (head, row) pairs of up to 32 chunks: 16 us in blocks of 256 threads
+// per 64 channels, 8 this way), W = 4 for longer ones.  grid (8 / W) (head, row, 64 channels) per block of 256 (W = 1) or 1 per block of 128
 template <int HD, class T, int W>
 __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_merge_k(Kv8Dev c, AttnArgs a) {
     __shared__ float2 part[W][32];
